@@ -80,7 +80,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   constexpr int kTileM = 256;
   constexpr int kAccStride = kOverlap ? 192 : 256;  // TMEM columns between the accumulators
   constexpr int kTmemCols = 512;
-  constexpr int kOutBN = (EPI == kEpiSwiGLU) ? BN / 2 : BN;
+  constexpr int kOutBN = epi_glu(EPI) ? BN / 2 : BN;
   constexpr bool kTmaStoreOk = kOutBN % 64 == 0;  // output boxes are 64 columns wide
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -358,7 +358,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           kScaled ? p.col_scale + static_cast<size_t>(info.seg % p.num_experts) * p.n_b : nullptr;
       // overlapped accumulators: the columns shared with the other accumulator first (the last
       // 64 of accumulator 0, the first 64 of accumulator 1), then release the next tile's MMAs
-      constexpr int kBoxes = (EPI == kEpiSwiGLU ? BN / 2 : BN) / 64;
+      constexpr int kBoxes = kOutBN / 64;
       store_tile_rows<BN, EPI, BF16>(t_row, info.n0, p.n_out, row_ok, out_row, warp_tma, &tmC,
                                      staging + ew * 4096, info.row0 + wrow0, rs, cs_row,
                                      p.n_b / 2, p.origin != nullptr,
