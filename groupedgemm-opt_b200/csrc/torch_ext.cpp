@@ -7,6 +7,7 @@
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
@@ -34,6 +35,12 @@ int dtype_code(const torch::Tensor& t) {
   return -1;
 }
 
+bool capturing(cudaStream_t stream) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  TORCH_CHECK(cudaStreamIsCapturing(stream, &st) == cudaSuccess, "capture status");
+  return st != cudaStreamCaptureStatusNone;
+}
+
 // One zero-initialised workspace per (device, stream); kept for the life of the process.
 std::mutex g_ws_mu;
 std::map<std::pair<int, cudaStream_t>, torch::Tensor> g_ws;
@@ -43,8 +50,23 @@ void* workspace_for(const torch::Device& dev, cudaStream_t stream) {
   auto key = std::make_pair(static_cast<int>(dev.index()), stream);
   auto it = g_ws.find(key);
   if (it == g_ws.end()) {
-    auto t = torch::zeros({static_cast<int64_t>(ggo_workspace_size())},
-                          torch::TensorOptions().dtype(torch::kUInt8).device(dev));
+    const auto opts = torch::TensorOptions().dtype(torch::kUInt8).device(dev);
+    const int64_t bytes = static_cast<int64_t>(ggo_workspace_size());
+    torch::Tensor t;
+    if (capturing(stream)) {
+      // The first call on this stream is a captured one. The workspace outlives the graph and is
+      // used outside it too, so it must neither come from the graph's memory pool nor be zeroed by
+      // a node of the graph: make it on a stream that is not being captured, and wait for it.
+      c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+      c10::cuda::CUDAStream side = c10::cuda::getStreamFromPool(false, dev.index());
+      for (int i = 0; i < 64 && capturing(side); ++i)
+        side = c10::cuda::getStreamFromPool(false, dev.index());
+      c10::cuda::CUDAStreamGuard on_side(side);
+      t = torch::zeros({bytes}, opts);
+      TORCH_CHECK(cudaStreamSynchronize(side) == cudaSuccess, "workspace set-up");
+    } else {
+      t = torch::zeros({bytes}, opts);
+    }
     it = g_ws.emplace(key, t).first;
   }
   return it->second.data_ptr();
