@@ -70,8 +70,9 @@ int make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t k, bool bf1
                      box_rows, box_cols);
 }
 
-// Operand map for 1-byte e4m3 data: rows of K bytes, boxes of 128 elements (128 B) x box_rows.
-int make_map_fp8(CUtensorMap* m, const void* base, int64_t rows, int64_t k, int box_rows) {
+// Operand map for 1-byte data (e4m3, int8): rows of K bytes, boxes of 128 elements (128 B) x
+// box_rows.
+int make_map_byte(CUtensorMap* m, const void* base, int64_t rows, int64_t k, int box_rows) {
   return make_map_dt(m, base, rows, k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, box_rows, 128);
 }
 
@@ -139,15 +140,15 @@ int make_b_map(CUtensorMap* m, const void* b, int64_t b_rows, const GemmParams& 
   return make_map(m, b, b_rows, q.k, bf16, box_rows);
 }
 
-template <int BN, int EPI, bool BF16, bool BMN = false, bool FP8 = false>
+template <int BN, int EPI, bool BF16, bool BMN = false, int OP = kOp16>
 int launch(const void* a, const void* b, int64_t b_rows, const GemmParams& p, int dev,
            cudaStream_t stream) {
   CUtensorMap ma, mb, mc, mas;
   memset(&mas, 0, sizeof(mas));
   GemmParams q = p;
-  if (FP8) {
-    if (int st = make_map_fp8(&ma, a, q.rows, q.k, kBM)) return st;
-    if (int st = make_map_fp8(&mb, b, b_rows, q.k, 128)) return st;
+  if (OP != kOp16) {
+    if (int st = make_map_byte(&ma, a, q.rows, q.k, kBM)) return st;
+    if (int st = make_map_byte(&mb, b, b_rows, q.k, 128)) return st;
     q.skinny_max = 0;
   } else {
     if (int st = make_map(&ma, a, q.rows, q.k, BF16, kBM)) return st;
@@ -159,7 +160,7 @@ int launch(const void* a, const void* b, int64_t b_rows, const GemmParams& p, in
     }
   }
   if (int st = make_out_map(&mc, &q, BF16)) return st;
-  auto kern = grouped_gemm_kernel<BN, EPI, BF16, BMN, FP8>;
+  auto kern = grouped_gemm_kernel<BN, EPI, BF16, BMN, OP>;
   constexpr int smem = SmemLayout<BN>::kTotal;
   int sms = 0;
   if (int st = kernel_setup(kern, smem, dev, false, &sms)) return st;
@@ -180,7 +181,7 @@ struct MxScales {
   int64_t b_atoms = 0;
 };
 
-template <int BN, int EPI, bool BF16, bool BMN = false, bool FP8 = false, bool MX = false>
+template <int BN, int EPI, bool BF16, bool BMN = false, int OP = kOp16, bool MX = false>
 int launch_pair(const void* a, const void* b, int64_t b_rows, const GemmParams& p, int dev,
                 cudaStream_t stream, const MxScales* mx = nullptr) {
   CUtensorMap ma, mb, mc, msa, msb;
@@ -192,15 +193,15 @@ int launch_pair(const void* a, const void* b, int64_t b_rows, const GemmParams& 
     if (int st = make_sf_map(&msb, mx->b, mx->b_atoms)) return st;
   }
   GemmParams q = p;
-  if (FP8) {
-    if (int st = make_map_fp8(&ma, a, q.rows, q.k, 128)) return st;
-    if (int st = make_map_fp8(&mb, b, b_rows, q.k, BN / 2)) return st;
+  if (OP != kOp16) {
+    if (int st = make_map_byte(&ma, a, q.rows, q.k, 128)) return st;
+    if (int st = make_map_byte(&mb, b, b_rows, q.k, BN / 2)) return st;
   } else {
     if (int st = make_map(&ma, a, q.rows, q.k, BF16, 128)) return st;
     if (int st = make_b_map<BMN>(&mb, b, b_rows, q, BF16, BN / 2)) return st;
   }
   if (int st = make_out_map(&mc, &q, BF16)) return st;
-  auto kern = grouped_gemm_pair_kernel<BN, EPI, BF16, BMN, FP8, MX>;
+  auto kern = grouped_gemm_pair_kernel<BN, EPI, BF16, BMN, OP, MX>;
   constexpr int smem = PairLayout<BN, MX>::kTotal;
   int clusters = 0;
   if (int st = kernel_setup(kern, smem, dev, true, &clusters)) return st;
@@ -302,6 +303,8 @@ struct GemmExtras {
   int world = 1;
   // FP8 path: e4m3 operands, out = acc * row_scale[row] * col_scale[expert * n + col] in bf16
   int fp8 = 0;
+  // INT8 path: signed 8-bit operands, the same scaled epilogue, out in bf16 or fp16
+  int i8 = 0;
   const float* row_scale = nullptr;
   const float* col_scale = nullptr;
   // MX path (with fp8): e4m3 operands with UE8M0 block scales (one per 32 K elements) in the
@@ -309,6 +312,7 @@ struct GemmExtras {
   int mx = 0;
   const void* a_sf = nullptr;
   const void* b_sf = nullptr;
+  int* err = nullptr;  // where device errors go (nullptr: the workspace's own error word)
 };
 
 // MX tiles: CTA pairs of 256 x 256 with overlapping accumulators (TMEM columns 0-255 and
@@ -321,6 +325,26 @@ int64_t mx_glu_rows(int64_t f) { return 2 * ((f + kMxGluBlock - 1) / kMxGluBlock
 // 512-B scale atoms of `rows` rows in `segments` segments (each padded to 128 rows), K columns
 int64_t mx_scale_atoms(int64_t rows, int64_t segments, int64_t k) {
   return ((rows + 127) / 128 + segments) * (k / 128);
+}
+
+// One-byte operands with the scaled epilogue: CTA-pair pass (+ short-tail pass) or single-CTA
+// 128x256 tiles.
+template <int EPI, bool BF16, int OP>
+int launch_scaled(const void* input, const void* weights, int64_t b_rows, GemmParams p, int bn,
+                  int dev, cudaStream_t stream) {
+  if (bn == 512) {
+    const bool split = env_int("GGO_SPLIT_TAILS", 1) > 0;
+    const int out_bn = epi_glu(EPI) ? 128 : 256;
+    p.split_tail_ntiles = (p.n_out + out_bn - 1) / out_bn;
+    p.split_min_tiles = env_int("GGO_SPLIT_MIN_TILES", 2 * g_sm_count[dev]);
+    GemmParams pp = p;
+    pp.group_m = raster_group_m(p.k / 2, 256);  // k bytes: half the bf16 panel size
+    pp.split_mode = split ? 1 : 0;
+    const int st = launch_pair<256, EPI, BF16, false, OP>(input, weights, b_rows, pp, dev, stream);
+    if (st || !split) return st;
+    p.split_mode = 2;
+  }
+  return launch<256, EPI, BF16, false, OP>(input, weights, b_rows, p, dev, stream);
 }
 
 int gemm_common(const void* input, const void* weights, void* output, const int64_t* counts,
@@ -342,6 +366,7 @@ int gemm_common(const void* input, const void* weights, void* output, const int6
   if (num_segments > kMaxSegments) return GGO_ERR_TOO_MANY_SEGMENTS;
   const bool fp8 = ex && ex->fp8;
   const bool mx = fp8 && ex->mx;
+  const bool i8 = ex && ex->i8;
   if (fp8) {
     if (bmn || scatter) return GGO_ERR_INVALID_ARG;
     if (mx ? (!ex->a_sf || !ex->b_sf) : (!ex->row_scale || !ex->col_scale))
@@ -349,6 +374,12 @@ int gemm_common(const void* input, const void* weights, void* output, const int6
     dtype = GGO_DTYPE_BF16;  // e4m3 in, bf16 out
     if (k % (mx ? 128 : 16)) return GGO_ERR_ALIGNMENT;  // rows of K bytes; MX: whole scale atoms
     if (mx && (!aligned16(ex->a_sf) || !aligned16(ex->b_sf))) return GGO_ERR_ALIGNMENT;
+  }
+  if (i8) {
+    if (!ex->row_scale || !ex->col_scale) return GGO_ERR_INVALID_ARG;
+    if (k % 16) return GGO_ERR_ALIGNMENT;  // rows of K bytes
+    // |sum of k products of signed bytes| <= k * 2^14 has to stay inside 32 bits
+    if (k > GGO_INT8_MAX_K) return GGO_ERR_SHAPE;
   }
   if (dtype != GGO_DTYPE_BF16 && dtype != GGO_DTYPE_FP16) return GGO_ERR_DTYPE;
   if ((k % 8) || (n % 8)) return GGO_ERR_ALIGNMENT;
@@ -389,12 +420,13 @@ int gemm_common(const void* input, const void* weights, void* output, const int6
     p.skinny_max = v < 0 ? 0 : (v > kSkinnyRows ? kSkinnyRows : v);
   }
   p.rows_is_bound = ex ? ex->rows_is_bound : 0;
-  p.row_scale = fp8 ? ex->row_scale : nullptr;
-  p.col_scale = fp8 ? ex->col_scale : nullptr;
+  p.row_scale = (fp8 || i8) ? ex->row_scale : nullptr;
+  p.col_scale = (fp8 || i8) ? ex->col_scale : nullptr;
   p.origin = scatter ? ex->origin : nullptr;
   for (int r = 0; r < 8; ++r) p.peer_out[r] = (scatter && r < ex->world) ? ex->peer_out[r] : nullptr;
   p.out = output;
   p.ws = static_cast<GgoWorkspace*>(workspace);
+  p.err = ex && ex->err ? ex->err : &p.ws->error;
   const bool bf16 = dtype == GGO_DTYPE_BF16;
   int bn = choose_bn(tile_config, rows, swiglu ? 2 * n : n, num_segments, g_sm_count[dev]);
   if (mx) {  // CTA pairs only (no short-tail pass: its scales would need a second layout)
@@ -411,32 +443,26 @@ int gemm_common(const void* input, const void* weights, void* output, const int6
       return GGO_ERR_SHAPE;
     p.group_m = raster_group_m(k / 2, 256);
     p.glu_blocked = swiglu ? 1 : 0;
-    return swiglu ? launch_pair<kMxPairBN, kEpiSwiGLU, true, false, true, true>(
+    return swiglu ? launch_pair<kMxPairBN, kEpiSwiGLU, true, false, kOpE4M3, true>(
                         input, weights, b_rows, p, dev, stream, &sc)
-                  : launch_pair<kMxPairBN, kEpiStore, true, false, true, true>(
+                  : launch_pair<kMxPairBN, kEpiStore, true, false, kOpE4M3, true>(
                         input, weights, b_rows, p, dev, stream, &sc);
   }
-  if (fp8) {  // CTA-pair pass (+ short-tail pass) or single-CTA 128x256, scaled epilogue
-    if (bn == 512) {
-      const bool split = env_int("GGO_SPLIT_TAILS", 1) > 0;
-      p.split_tail_ntiles = static_cast<int>((n + (swiglu ? 127 : 255)) / (swiglu ? 128 : 256));
-      p.split_min_tiles = env_int("GGO_SPLIT_MIN_TILES", 2 * g_sm_count[dev]);
-      GemmParams pp = p;
-      pp.group_m = raster_group_m(k / 2, 256);  // k bytes: half the bf16 panel size
-      pp.split_mode = split ? 1 : 0;
-      const int st =
-          swiglu ? launch_pair<256, kEpiScaledSwiGLU, true, false, true>(input, weights, b_rows,
-                                                                         pp, dev, stream)
-                 : launch_pair<256, kEpiScaled, true, false, true>(input, weights, b_rows, pp, dev,
-                                                                   stream);
-      if (st) return st;
-      if (!split) return GGO_OK;
-      p.split_mode = 2;
-    }
-    return swiglu
-               ? launch<256, kEpiScaledSwiGLU, true, false, true>(input, weights, b_rows, p, dev,
-                                                                  stream)
-               : launch<256, kEpiScaled, true, false, true>(input, weights, b_rows, p, dev, stream);
+  if (fp8) {
+    return swiglu ? launch_scaled<kEpiScaledSwiGLU, true, kOpE4M3>(input, weights, b_rows, p, bn,
+                                                                   dev, stream)
+                  : launch_scaled<kEpiScaled, true, kOpE4M3>(input, weights, b_rows, p, bn, dev,
+                                                             stream);
+  }
+  if (i8) {
+    if (swiglu)
+      return bf16 ? launch_scaled<kEpiScaledSwiGLU, true, kOpI8>(input, weights, b_rows, p, bn,
+                                                                 dev, stream)
+                  : launch_scaled<kEpiScaledSwiGLU, false, kOpI8>(input, weights, b_rows, p, bn,
+                                                                  dev, stream);
+    return bf16 ? launch_scaled<kEpiScaled, true, kOpI8>(input, weights, b_rows, p, bn, dev, stream)
+                : launch_scaled<kEpiScaled, false, kOpI8>(input, weights, b_rows, p, bn, dev,
+                                                          stream);
   }
   if (bn == 512) {
     // CTA-pair pass over 256-row tiles, then (GGO_SPLIT_TAILS, default on) a single-CTA pass over
@@ -699,6 +725,26 @@ int ggo_grouped_gemm_swiglu_fp8(const void* x_dev, const float* x_scale_dev,
   return ggo::gemm_common(x_dev, w_gate_up_dev, h_dev, tokens_per_segment_dev, num_segments,
                           num_experts, total_tokens, F, K, GGO_DTYPE_BF16, GGO_TILE_AUTO,
                           sort_by_m, workspace_dev, stream, true, &ex);
+}
+
+int ggo_grouped_gemm_int8(const void* input_dev, const float* input_scale_dev,
+                          const void* weights_dev, const float* weight_scale_dev,
+                          void* output_dev, const int64_t* tokens_per_segment_dev,
+                          int num_segments, int num_experts, int64_t total_tokens, int64_t N,
+                          int64_t K, int out_dtype, int swiglu, int tile_config, int sort_by_m,
+                          void* workspace_dev, int* error_dev, cudaStream_t stream) {
+  ggo::GemmExtras ex;
+  ex.i8 = 1;
+  ex.row_scale = input_scale_dev;
+  ex.col_scale = weight_scale_dev;
+  ex.err = error_dev;
+  return ggo::gemm_common(input_dev, weights_dev, output_dev, tokens_per_segment_dev, num_segments,
+                          num_experts, total_tokens, N, K, out_dtype, tile_config, sort_by_m,
+                          workspace_dev, stream, swiglu != 0, &ex);
+}
+
+int* ggo_workspace_error_word(void* workspace_dev) {
+  return workspace_dev ? &static_cast<ggo::GgoWorkspace*>(workspace_dev)->error : nullptr;
 }
 
 size_t ggo_mxfp8_scale_bytes(int64_t rows, int num_segments, int64_t k) {

@@ -21,7 +21,7 @@
 //    one 256-wide B tile holds 128 gate rows and the matching 128 up rows; row/column-scaled for
 //    FP8 operands; and a scatter of each row to its source rank's buffer (expert parallelism).
 //  * Operand forms: K-major weights (forward), MN-major weights read in place (dgrad), bf16/fp16
-//    (kind::f16) or e4m3 (kind::f8f6f4).
+//    (kind::f16), e4m3 (kind::f8f6f4) or signed 8-bit integers (kind::i8).
 //  * The CTA-pair variant (ggo_gemm_pair.cuh) shares the segment table, tile decode and epilogue.
 //
 // Every bulk-tensor load writes only the issuing CTA's shared memory, from this GPU's memory.
@@ -43,8 +43,11 @@ constexpr int kMaxSegments = 1024;
 constexpr int kSchedDepth = 4;
 constexpr int kThreads = 256;
 
-// kEpiScaled: out = acc * row_scale[row] * col_scale[expert * n_out + col] (the FP8 path).
-// kEpiScaledSwiGLU: silu(gate * rs * cs_gate) * (up * rs * cs_up) (the FP8 gate/up projection).
+// Operand element types of the GEMM kernels (template parameter OP).
+enum OpKind { kOp16 = 0, kOpE4M3 = 1, kOpI8 = 2 };
+
+// kEpiScaled: out = acc * row_scale[row] * col_scale[expert * n_out + col] (the FP8 and INT8 paths).
+// kEpiScaledSwiGLU: silu(gate * rs * cs_gate) * (up * rs * cs_up) (their gate/up projections).
 enum EpiKind { kEpiStore = 0, kEpiSwiGLU = 1, kEpiScaled = 2, kEpiScaledSwiGLU = 3 };
 
 // Epilogues whose B tile is [gate rows | up rows] and whose output is half the tile width.
@@ -105,6 +108,7 @@ struct GemmParams {
   // 128-row block. 0 disables. Single-CTA kernel, bf16/fp16 K-major weights, plain or SwiGLU.
   int skinny_max;
   GgoWorkspace* ws;
+  int* err;  // where device errors are recorded (first one wins): &ws->error unless given apart
 };
 
 constexpr int kSkinnyRows = 64;  // rows of the input box a skinny tile loads (its row limit)
@@ -371,7 +375,14 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
 
 // 32 output columns of this thread's accumulator row, packed as 16 bf16x2/half2 words: TMEM
 // columns [c, c+32) (plain), or silu(gate) * up from columns [c, c+32) and [BN/2 + c, ...).
-template <int BN, int EPI, bool BF16>
+// An accumulator word as fp32: already fp32, or (I8) a 32-bit integer sum, rounded to nearest (exact
+// up to 2^24).
+template <bool I8>
+__device__ __forceinline__ float acc_to_float(uint32_t v) {
+  return I8 ? __int2float_rn(static_cast<int>(v)) : __uint_as_float(v);
+}
+
+template <int BN, int EPI, bool BF16, bool I8 = false>
 __device__ __forceinline__ void load_out32(uint32_t t_row, int c, uint32_t (&o)[16], float rs = 1.f,
                                            const float* cs = nullptr, int cs_valid = 0,
                                            int cs_up_off = 0) {
@@ -387,8 +398,8 @@ __device__ __forceinline__ void load_out32(uint32_t t_row, int c, uint32_t (&o)[
       for (int e = 0; e < 2; ++e) {
         const int j = 2 * i + e;
         const bool ok = j < cs_valid;
-        const float gv = __uint_as_float(g[j]) * rs * (ok ? __ldg(cs + j) : 0.f);
-        const float uv = __uint_as_float(u[j]) * rs * (ok ? __ldg(cs + cs_up_off + j) : 0.f);
+        const float gv = acc_to_float<I8>(g[j]) * rs * (ok ? __ldg(cs + j) : 0.f);
+        const float uv = acc_to_float<I8>(u[j]) * rs * (ok ? __ldg(cs + cs_up_off + j) : 0.f);
         y[e] = gv / (1.0f + __expf(-gv)) * uv;
       }
       o[i] = pack2(y[0], y[1], BF16);
@@ -401,8 +412,8 @@ __device__ __forceinline__ void load_out32(uint32_t t_row, int c, uint32_t (&o)[
     for (int i = 0; i < 16; ++i) {
       const float s0 = 2 * i < cs_valid ? __ldg(cs + 2 * i) : 0.f;
       const float s1 = 2 * i + 1 < cs_valid ? __ldg(cs + 2 * i + 1) : 0.f;
-      o[i] = pack2(__uint_as_float(v[2 * i]) * rs * s0, __uint_as_float(v[2 * i + 1]) * rs * s1,
-                   BF16);
+      o[i] = pack2(acc_to_float<I8>(v[2 * i]) * rs * s0,
+                   acc_to_float<I8>(v[2 * i + 1]) * rs * s1, BF16);
     }
   } else if (EPI == kEpiStore) {
     uint32_t v[32];
@@ -443,7 +454,7 @@ __device__ __forceinline__ void load_out32(uint32_t t_row, int c, uint32_t (&o)[
 //    contiguous bytes -- so each store instruction sends whole rows instead of 16-byte pieces of
 //    32 different rows.
 //  * otherwise each thread stores its own row with 16-byte stores, masked by row_ok and n_out.
-template <int BN, int EPI, bool BF16, typename OutT>
+template <int BN, int EPI, bool BF16, typename OutT, bool I8 = false>
 __device__ __forceinline__ void store_tile_rows(uint32_t t_row, int n0, int n_out, bool row_ok,
                                                 OutT* out_row, bool warp_tma,
                                                 const CUtensorMap* tmC, uint8_t* stage,
@@ -470,9 +481,9 @@ __device__ __forceinline__ void store_tile_rows(uint32_t t_row, int n0, int n_ou
     // adding up box after box.
     uint32_t o[32];
     const int f64 = 64 * first_box;
-    load_out32<BN, EPI, BF16>(t_row, f64, *reinterpret_cast<uint32_t(*)[16]>(o), rs,
+    load_out32<BN, EPI, BF16, I8>(t_row, f64, *reinterpret_cast<uint32_t(*)[16]>(o), rs,
                               cs_row ? cs_row + n0 + f64 : nullptr, n_out - (n0 + f64), cs_up_off);
-    load_out32<BN, EPI, BF16>(t_row, f64 + 32, *reinterpret_cast<uint32_t(*)[16]>(o + 16), rs,
+    load_out32<BN, EPI, BF16, I8>(t_row, f64 + 32, *reinterpret_cast<uint32_t(*)[16]>(o + 16), rs,
                               cs_row ? cs_row + n0 + f64 + 32 : nullptr, n_out - (n0 + f64 + 32),
                               cs_up_off);
     release();
@@ -496,10 +507,10 @@ __device__ __forceinline__ void store_tile_rows(uint32_t t_row, int n0, int n_ou
       }
       const int nx = 64 * ((first_box + b + 1) % kBoxes);
       if (b + 1 < kBoxes) {
-        load_out32<BN, EPI, BF16>(t_row, nx, *reinterpret_cast<uint32_t(*)[16]>(o), rs,
+        load_out32<BN, EPI, BF16, I8>(t_row, nx, *reinterpret_cast<uint32_t(*)[16]>(o), rs,
                                   cs_row ? cs_row + n0 + nx : nullptr, n_out - (n0 + nx),
                                   cs_up_off);
-        load_out32<BN, EPI, BF16>(t_row, nx + 32, *reinterpret_cast<uint32_t(*)[16]>(o + 16), rs,
+        load_out32<BN, EPI, BF16, I8>(t_row, nx + 32, *reinterpret_cast<uint32_t(*)[16]>(o + 16), rs,
                                   cs_row ? cs_row + n0 + nx + 32 : nullptr,
                                   n_out - (n0 + nx + 32), cs_up_off);
       }
@@ -519,7 +530,7 @@ __device__ __forceinline__ void store_tile_rows(uint32_t t_row, int n0, int n_ou
       const int c = c64 + 32 * s;
       if (c >= OUTW) break;
       uint32_t o[16];
-      load_out32<BN, EPI, BF16>(t_row, c, o, rs, cs_row ? cs_row + n0 + c : nullptr,
+      load_out32<BN, EPI, BF16, I8>(t_row, c, o, rs, cs_row ? cs_row + n0 + c : nullptr,
                                 n_out - (n0 + c), cs_up_off);
       if (staged) {
 #pragma unroll
@@ -615,7 +626,7 @@ __device__ __forceinline__ void store_skinny(uint32_t t_row, const GemmParams& p
   }
 }
 
-template <int BN, int EPI, bool BF16, bool BMN = false, bool FP8 = false>
+template <int BN, int EPI, bool BF16, bool BMN = false, int OP = kOp16>
 __global__ void __launch_bounds__(kThreads, 1)
     grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA,
                         const __grid_constant__ CUtensorMap tmB,
@@ -627,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kOutBN = epi_glu(EPI) ? BN / 2 : BN;
   constexpr bool kTmaStoreOk = kOutBN % 64 == 0;  // output boxes are 64 columns wide
   // skinny tiles: tmAs is the input map with kSkinnyRows-row boxes
-  constexpr bool kSkinnyOk = !FP8 && !BMN && (EPI == kEpiStore || EPI == kEpiSwiGLU);
+  constexpr bool kSkinnyOk = OP == kOp16 && !BMN && (EPI == kEpiStore || EPI == kEpiSwiGLU);
   constexpr int kSkinnyABytes = kSkinnyRows * kBK * 2;
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -653,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  int* err = &p.ws->error;
+  int* err = p.err;
 
   // ------------------------------------------------------------------ set-up
   if (threadIdx.x == 0) {
@@ -687,8 +698,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem_base = *tmem_slot;
   const int total_tiles = *total_tiles_s;
   const int heavy_tiles = total_tiles_s[1];
-  // K elements per pipeline stage: one 128-B swizzle row (64 bf16/fp16 or 128 e4m3)
-  constexpr int kStageK = FP8 ? 128 : kBK;
+  // K elements per pipeline stage: one 128-B swizzle row (64 bf16/fp16 or 128 one-byte ones)
+  constexpr int kStageK = OP == kOp16 ? kBK : 128;
   const int num_kb = (p.k + kStageK - 1) / kStageK;
 
   if (warp == 0) {
@@ -751,7 +762,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // -------------------------------------------------------------- MMA issuer
     if (lane == 0) {
       // e4m3 operands are format 0 of kind::f8f6f4, the same bits as f16 in kind::f16
-      constexpr uint32_t idesc = idesc_f16(kBM, BN, FP8 ? false : BF16, BMN);
+      constexpr uint32_t idesc = OP == kOpI8 ? idesc_i8(kBM, BN)
+                                             : idesc_f16(kBM, BN, OP == kOp16 && BF16, BMN);
       int stage = 0, phase = 0, q = 0, qphase = 0, acc = 0, aphase = 0;
       const uint32_t tiles_addr = smem_u32(tiles);
       while (true) {
@@ -797,7 +809,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {  // four 32-byte K steps per 128-byte stage row
-            if (FP8)
+            if (OP == kOpI8)
+              mma_i8_ss(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
+            else if (OP == kOpE4M3)
               mma_f8_ss(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
             else
               mma_f16_ss(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
@@ -842,7 +856,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // column scales: one per weight row, [E, n_b] (gate rows then up rows for SwiGLU)
       const float* cs_row =
           kScaled ? p.col_scale + static_cast<size_t>(info.seg % p.num_experts) * p.n_b : nullptr;
-      store_tile_rows<BN, EPI, BF16>(t_row, info.n0, p.n_out, row_ok, out_row, warp_tma, &tmC,
+      store_tile_rows<BN, EPI, BF16, OutT, OP == kOpI8>(t_row, info.n0, p.n_out, row_ok, out_row, warp_tma, &tmC,
                                      staging + ew * 4096, info.row0 + ew * 32, rs, cs_row,
                                      p.n_b / 2, p.origin != nullptr);
       tc_fence_before();

@@ -47,7 +47,7 @@ struct PairLayout {
 // MX = block-scaled e4m3 (kind::mxf8f6f4): tmSFA / tmSFB view the UE8M0 scales of A and B as
 // [atoms * 2, 256] bytes (512-B atoms of 128 rows x 4 scales, the 128x4 blocked layout: a
 // segment's rows start on a fresh 128-row block, atom (block, K group) at block * K/128 + group).
-template <int BN, int EPI, bool BF16, bool BMN = false, bool FP8 = false, bool MX = false>
+template <int BN, int EPI, bool BF16, bool BMN = false, int OP = kOp16, bool MX = false>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grouped_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA,
                              const __grid_constant__ CUtensorMap tmB,
@@ -63,7 +63,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   // multiples of their width inside an expert, so a width in {64, 128, 192} gives exactly those
   // offsets (256 leaves no TMEM columns for the scale slots). A 224-wide variant (N = 224, offsets
   // 1 and 3) stopped with a misaligned-address error and is not built.
-  static_assert(!MX || (FP8 && !BMN && (BN == 64 || BN == 128 || BN == 192 || BN == 256)),
+  static_assert(!MX || (OP == kOpE4M3 && !BMN && (BN == 64 || BN == 128 || BN == 192 || BN == 256)),
                 "MX tile width");
   static_assert(!MX || 4 + 4 * L::kSfbAtoms <= 16, "scale slot width");
   // MX with 256-wide tiles: the two accumulators overlap by 64 TMEM columns (columns 0-255 and
@@ -109,7 +109,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
-  int* err = &p.ws->error;
+  int* err = p.err;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
@@ -159,7 +159,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t tmem_base = *tmem_slot;
   const int total_tiles = *total_tiles_s;
   const int heavy_tiles = total_tiles_s[1];
-  constexpr int kStageK = FP8 ? 128 : kBK;  // K elements per stage (one 128-B swizzle row)
+  constexpr int kStageK = OP == kOp16 ? kBK : 128;  // K elements per stage (one 128-B swizzle row)
   const int num_kb = (p.k + kStageK - 1) / kStageK;
 
   if (warp == 0) {
@@ -251,7 +251,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     // -------------------------------------------------------------- MMA issuer (leader only)
     if (leader && lane == 0) {
-      constexpr uint32_t idesc = idesc_f16(kTileM, BN, FP8 ? false : BF16, BMN);
+      constexpr uint32_t idesc = OP == kOpI8 ? idesc_i8(kTileM, BN)
+                                             : idesc_f16(kTileM, BN, OP == kOp16 && BF16, BMN);
       static_assert(!BMN || (BN / 2) % 64 == 0, "MN-major B halves are whole 64-column boxes");
       int stage = 0, phase = 0, q = 0, qphase = 0, acc = 0, aphase = 0;
       uint32_t sf_slot = 0;  // MX: scale slot of the next K step
@@ -317,7 +318,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           } else {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {  // four 32-byte K steps per 128-byte stage row
-            if (FP8)
+            if (OP == kOpI8)
+              mma_i8_ss_pair(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
+            else if (OP == kOpE4M3)
               mma_f8_ss_pair(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
             else
               mma_f16_ss_pair(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
@@ -359,7 +362,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // overlapped accumulators: the columns shared with the other accumulator first (the last
       // 64 of accumulator 0, the first 64 of accumulator 1), then release the next tile's MMAs
       constexpr int kBoxes = kOutBN / 64;
-      store_tile_rows<BN, EPI, BF16>(t_row, info.n0, p.n_out, row_ok, out_row, warp_tma, &tmC,
+      store_tile_rows<BN, EPI, BF16, OutT, OP == kOpI8>(t_row, info.n0, p.n_out, row_ok, out_row, warp_tma, &tmC,
                                      staging + ew * 4096, info.row0 + wrow0, rs, cs_row,
                                      p.n_b / 2, p.origin != nullptr,
                                      kOverlap ? (acc == 0 ? kBoxes - 1 : 0) : 0,

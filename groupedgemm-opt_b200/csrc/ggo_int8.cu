@@ -1,0 +1,297 @@
+// INT8 quantisation of rows, alone and fused into the MoE dispatch.
+//
+// Signed 8-bit codes with one scale per row (token or output channel):
+//
+//   scale[r] = max|x[r, :]| / 127        q[r, c] = round_half_even(127 x[r, c] / max|x[r, :]|)
+//
+// (a zero row: scale 1, codes 0; a row with an infinity or NaN: scale NaN, codes 0, so everything
+// computed from the row is NaN). The code is defined by the quotient of 127 x and the maximum, not by
+// x / scale: with significands of at most 11 bits 127 x is exact in fp32, and a quotient in
+// [2^m, 2^(m+1)) that is not exactly half-way between two integers is at least 2^(m-20) away from
+// it, sixteen times fp32's half step there, so the fp32 quotient always rounds to the integer the
+// exact one rounds to. x / scale would inherit the rounding of the scale and miss the tie at
+// x = max / 2.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ggo.h"
+#include "ggo_internal.h"
+
+namespace ggo {
+namespace {
+
+constexpr unsigned kAll = 0xffffffffu;
+constexpr int kRouteTokens = 32;  // tokens per block of the router's offset table
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxTopK = 16;
+
+// Largest |x| of eight 16-bit floats as its bit pattern (for the sign-free patterns of one format
+// the order of the integers is the order of the values, NaN above infinity above all finite ones),
+// kept per 16-bit half.
+__device__ __forceinline__ uint32_t abs_max8(uint32_t m, const uint4& v) {
+  m = __vmaxu2(m, v.x & 0x7fff7fffu);
+  m = __vmaxu2(m, v.y & 0x7fff7fffu);
+  m = __vmaxu2(m, v.z & 0x7fff7fffu);
+  return __vmaxu2(m, v.w & 0x7fff7fffu);
+}
+
+template <typename T16>
+__device__ __forceinline__ float from_bits(uint32_t b) {
+  const unsigned short h = static_cast<unsigned short>(b);
+  return static_cast<float>(*reinterpret_cast<const T16*>(&h));
+}
+
+// What a row needs to turn its values into codes: q = round(x * mul / top), mul a power of two times
+// 127 that brings the quotient's operands near 1 (no overflow, no underflow of anything that
+// could round to a code other than 0), inv = 1 / top.
+struct RowCode {
+  float mul, top, inv, scale;
+};
+
+template <typename T16>
+__device__ __forceinline__ RowCode row_code(uint32_t max2) {
+  const uint32_t bits = max(max2 & 0xffffu, max2 >> 16);
+  const float amax = from_bits<T16>(bits);
+  RowCode c;
+  const int field = static_cast<int>(__float_as_uint(amax) >> 23);  // biased exponent of the maximum
+  if (bits == 0 || field == 255) {
+    c.mul = 0.f;  // codes 0 (the quotient below is then 0 or, for x = inf or NaN, masked)
+    c.top = c.inv = 1.f;
+    c.scale = bits == 0 ? 1.f : __int_as_float(0x7fc00000);
+    return c;
+  }
+  // 2^(127 - exponent field), between 2^-126 and 2^119 so that it and 127 times it are normal
+  // numbers: top lands in [2^-14, 4)
+  const int f = 254 - field;
+  const float two = __uint_as_float(static_cast<uint32_t>(f < 1 ? 1 : (f > 246 ? 246 : f)) << 23);
+  c.top = amax * two;
+  c.mul = 127.f * two;
+  c.inv = __frcp_rn(c.top);
+  c.scale = __fdiv_rn(amax, 127.f);
+  return c;
+}
+
+// Code of x as the low byte of the result. t = 127 x and top are exact, and one correction of
+// q0 = t * (1 / top) with the exact remainder r = t - top q0 gives the correctly rounded quotient
+// (Markstein, IBM J. Res. Dev. 34(1), 1990). Adding 1.5 * 2^23 rounds it to an integer, half to even, whose
+// two's complement is the sum's low bits.
+__device__ __forceinline__ uint32_t code_of(float x, const RowCode& c) {
+  const float t = x * c.mul;
+  const float q0 = t * c.inv;
+  const float q = fmaf(fmaf(-c.top, q0, t), c.inv, q0);
+  return __float_as_uint(q + 12582912.f);
+}
+
+// Eight values to eight codes (64 bits).
+template <typename T16>
+__device__ __forceinline__ uint2 code8(const uint4& v, const RowCode& c) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t o[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t a = code_of(from_bits<T16>(w[2 * h] & 0xffffu), c);
+    const uint32_t b = code_of(from_bits<T16>(w[2 * h] >> 16), c);
+    const uint32_t d = code_of(from_bits<T16>(w[2 * h + 1] & 0xffffu), c);
+    const uint32_t e = code_of(from_bits<T16>(w[2 * h + 1] >> 16), c);
+    o[h] = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(d, e, 0x0040), 0x5410);
+  }
+  return c.mul == 0.f ? make_uint2(0u, 0u) : make_uint2(o[0], o[1]);
+}
+
+__device__ __forceinline__ uint32_t warp_max2(uint32_t m) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(kAll, m, o));
+  return m;
+}
+
+// One 256-thread block per row, the row held in registers (cols <= kRegCols).
+constexpr int kVec = 8;
+constexpr int kRegCols = 256 * kVec * 8;  // 16384
+
+template <typename T16>
+__global__ void __launch_bounds__(256)
+    quantize_int8_block_kernel(const T16* __restrict__ x, int cols, uint8_t* __restrict__ q,
+                               float* __restrict__ scale) {
+  __shared__ uint32_t s_max[8];
+  const size_t r = blockIdx.x;
+  const int vec = cols / 8;
+  const uint4* xr = reinterpret_cast<const uint4*>(x + r * cols);
+  uint4 v[kVec];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    const int c = threadIdx.x + i * 256;
+    v[i] = c < vec ? xr[c] : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) m = abs_max8(m, v[i]);
+  m = warp_max2(m);
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = __vmaxu2(m, s_max[w]);
+  const RowCode rc = row_code<T16>(m);
+  if (threadIdx.x == 0) scale[r] = rc.scale;
+  uint2* qr = reinterpret_cast<uint2*>(q + r * cols);
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    const int c = threadIdx.x + i * 256;
+    if (c < vec) qr[c] = code8<T16>(v[i], rc);
+  }
+}
+
+// Rows longer than the block form holds: two passes, the second one out of L2.
+template <typename T16>
+__global__ void __launch_bounds__(256)
+    quantize_int8_long_kernel(const T16* __restrict__ x, int cols, uint8_t* __restrict__ q,
+                              float* __restrict__ scale) {
+  __shared__ uint32_t s_max[8];
+  const size_t r = blockIdx.x;
+  const int vec = cols / 8;
+  const uint4* xr = reinterpret_cast<const uint4*>(x + r * cols);
+  uint32_t m = 0;
+#pragma unroll 4
+  for (int c = threadIdx.x; c < vec; c += 256) m = abs_max8(m, xr[c]);
+  m = warp_max2(m);
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = __vmaxu2(m, s_max[w]);
+  const RowCode rc = row_code<T16>(m);
+  if (threadIdx.x == 0) scale[r] = rc.scale;
+  uint2* qr = reinterpret_cast<uint2*>(q + r * cols);
+#pragma unroll 4
+  for (int c = threadIdx.x; c < vec; c += 256) qr[c] = code8<T16>(xr[c], rc);
+}
+
+// The dispatch's permutation with the quantisation on the way: every token's row is read, coded
+// once and written to its top_k expert-sorted places as codes. grid = (ceil(T / 32), kSplit): block
+// (b, s) finds the sorted positions of 32-token block b (one warp walks its (token, slot) entries
+// in order, as the bf16 dispatch does) and moves the tokens congruent to s mod kSplit, one warp each.
+constexpr int kSplit = 4;
+
+template <typename T16>
+__global__ void __launch_bounds__(256)
+    permute_int8_kernel(const T16* __restrict__ x, int T, int H, int E, int K,
+                        const int32_t* __restrict__ topk_ids, const int* __restrict__ block_offsets,
+                        uint8_t* __restrict__ q_sorted, float* __restrict__ scale_sorted,
+                        int32_t* __restrict__ slot_pos) {
+  extern __shared__ int psm[];
+  int* off = psm;      // [E] running sorted position per expert
+  int* pos = psm + E;  // [kRouteTokens * K]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t0 = blockIdx.x * kRouteTokens;
+  const int ntok = min(kRouteTokens, T - t0);
+  const int nent = ntok * K;
+  for (int e = threadIdx.x; e < E; e += 256)
+    off[e] = block_offsets[static_cast<size_t>(blockIdx.x) * E + e];
+  __syncthreads();
+  if (warp == 0) {
+    const int32_t* ids = topk_ids + static_cast<size_t>(t0) * K;
+    for (int base = 0; base < nent; base += 32) {
+      const int i = base + lane;
+      const bool valid = i < nent;
+      const unsigned vmask = __ballot_sync(kAll, valid);
+      if (valid) {
+        const int id = ids[i];
+        const unsigned peers = __match_any_sync(vmask, id);
+        const int b = off[id];
+        __syncwarp(vmask);
+        if (lane == __ffs(peers) - 1) off[id] = b + __popc(peers);
+        const int ps = b + __popc(peers & ((1u << lane) - 1u));
+        pos[i] = ps;
+        if (blockIdx.y == 0) slot_pos[static_cast<size_t>(t0) * K + i] = ps;
+      }
+      __syncwarp();
+    }
+  }
+  __syncthreads();
+  const int vec = H / 8;
+  for (int tl = warp * kSplit + blockIdx.y; tl < ntok; tl += 8 * kSplit) {
+    const uint4* src = reinterpret_cast<const uint4*>(x + static_cast<size_t>(t0 + tl) * H);
+    uint32_t m = 0;
+#pragma unroll 8
+    for (int c = lane; c < vec; c += 32) m = abs_max8(m, src[c]);
+    const RowCode rc = row_code<T16>(warp_max2(m));
+    for (int j = lane; j < K; j += 32) scale_sorted[pos[tl * K + j]] = rc.scale;
+#pragma unroll 4
+    for (int c = lane; c < vec; c += 32) {
+      const uint2 o = code8<T16>(src[c], rc);
+      for (int j = 0; j < K; ++j)
+        reinterpret_cast<uint2*>(q_sorted + static_cast<size_t>(pos[tl * K + j]) * H)[c] = o;
+    }
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <typename T16>
+int launch_quantize(const void* x, int64_t rows, int cols, uint8_t* q, float* scale,
+                    cudaStream_t stream) {
+  const T16* xp = static_cast<const T16*>(x);
+  if (cols <= kRegCols)
+    quantize_int8_block_kernel<T16><<<static_cast<unsigned>(rows), 256, 0, stream>>>(xp, cols, q,
+                                                                                  scale);
+  else
+    quantize_int8_long_kernel<T16><<<static_cast<unsigned>(rows), 256, 0, stream>>>(xp, cols, q,
+                                                                                 scale);
+  return check_launch();
+}
+
+template <typename T16>
+int launch_permute(const void* x, int T, int H, int E, int K, const int32_t* ids,
+                   const int* offsets, uint8_t* q, float* scale, int32_t* slot_pos,
+                   cudaStream_t stream) {
+  const dim3 grid((T + kRouteTokens - 1) / kRouteTokens, kSplit);
+  const size_t smem = (static_cast<size_t>(E) + kRouteTokens * K) * 4;  // at most 6 KB
+  permute_int8_kernel<T16><<<grid, 256, smem, stream>>>(static_cast<const T16*>(x), T, H, E, K, ids,
+                                                        offsets, q, scale, slot_pos);
+  return check_launch();
+}
+
+}  // namespace
+}  // namespace ggo
+
+extern "C" {
+
+int ggo_quantize_int8_rows(const void* x_dev, int64_t rows, int64_t cols, int dtype, void* q_dev,
+                           float* scale_dev, cudaStream_t stream) {
+  if (rows < 0 || cols <= 0) return GGO_ERR_INVALID_ARG;
+  if (dtype != GGO_DTYPE_BF16 && dtype != GGO_DTYPE_FP16) return GGO_ERR_DTYPE;
+  if (rows == 0) return GGO_OK;
+  if (!x_dev || !q_dev || !scale_dev) return GGO_ERR_INVALID_ARG;
+  if (cols % 16 || !ggo::aligned16(x_dev) || !ggo::aligned16(q_dev)) return GGO_ERR_ALIGNMENT;
+  if (rows > INT32_MAX || cols > INT32_MAX) return GGO_ERR_SHAPE;
+  uint8_t* q = static_cast<uint8_t*>(q_dev);
+  const int c = static_cast<int>(cols);
+  return dtype == GGO_DTYPE_BF16
+             ? ggo::launch_quantize<__nv_bfloat16>(x_dev, rows, c, q, scale_dev, stream)
+             : ggo::launch_quantize<__half>(x_dev, rows, c, q, scale_dev, stream);
+}
+
+int ggo_moe_permute_int8(const void* x_dev, int64_t num_tokens, int64_t hidden, int num_experts,
+                         int top_k, const int32_t* topk_ids_dev, void* q_sorted_dev,
+                         float* scale_sorted_dev, int32_t* slot_pos_dev, const void* scratch_dev,
+                         int dtype, cudaStream_t stream) {
+  if (num_tokens < 0 || hidden <= 0 || num_experts <= 0 || num_experts > ggo::kMaxExperts ||
+      top_k <= 0 || top_k > ggo::kMaxTopK || top_k > num_experts)
+    return GGO_ERR_INVALID_ARG;
+  if (dtype != GGO_DTYPE_BF16 && dtype != GGO_DTYPE_FP16) return GGO_ERR_DTYPE;
+  if (num_tokens == 0) return GGO_OK;
+  if (!x_dev || !topk_ids_dev || !q_sorted_dev || !scale_sorted_dev || !slot_pos_dev ||
+      !scratch_dev)
+    return GGO_ERR_INVALID_ARG;
+  if (hidden % 16 || !ggo::aligned16(x_dev) || !ggo::aligned16(q_sorted_dev))
+    return GGO_ERR_ALIGNMENT;
+  if (num_tokens * top_k > INT32_MAX || hidden > INT32_MAX) return GGO_ERR_SHAPE;
+  const int T = static_cast<int>(num_tokens), H = static_cast<int>(hidden);
+  uint8_t* q = static_cast<uint8_t*>(q_sorted_dev);
+  const int* off = static_cast<const int*>(scratch_dev);
+  return dtype == GGO_DTYPE_BF16
+             ? ggo::launch_permute<__nv_bfloat16>(x_dev, T, H, num_experts, top_k, topk_ids_dev, off,
+                                                  q, scale_sorted_dev, slot_pos_dev, stream)
+             : ggo::launch_permute<__half>(x_dev, T, H, num_experts, top_k, topk_ids_dev, off, q,
+                                           scale_sorted_dev, slot_pos_dev, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,444 @@
+// Router with balance loss, forward and backward.
+//
+// For every token t: the top_k experts of the fp32 logits l (ties to the lower index), their
+// softmax weights, and the softmax P over ALL experts. Over the kept tokens (not masked, at least
+// one logit above -inf; T' of them), with n_e the kept choices that fell on expert e:
+//
+//   f_e = n_e / (top_k T')     p_e = (1/T') sum_t P[t, e]     loss = E sum_e f_e p_e
+//
+// (1 for a balanced router). f is piecewise constant, so with g the loss's upstream gradient
+//
+//   d/dl[t, e] = g (E/T') P[t, e] (f_e - sum_e' P[t, e'] f_e')          (kept tokens)
+//              + w_j (u_j - sum_j' w_j' u_j')   where e is token t's choice j, u = grad of w.
+//
+// Nothing here is accumulated by floating-point atomics: counts are integers, the sums over tokens
+// go warp -> block -> a fixed-order reduction in 64 bits, so equal inputs give equal bits.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ggo.h"
+#include "ggo_internal.h"
+
+namespace ggo {
+namespace {
+
+constexpr int kTokens = 32;    // tokens per block: the granularity of the dispatch's offset table
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxE = 1024;
+constexpr int kMaxK = 16;
+constexpr unsigned kAll = 0xffffffffu;
+
+// Monotone float -> uint32 (larger float -> larger key). -0 counts as +0 and NaN as the largest, so
+// that equal floats have equal keys; 0 is below every key and marks a chosen or absent expert.
+__device__ __forceinline__ uint32_t order_key(float f) {
+  if (f != f) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(f + 0.0f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  if (k == 0xffffffffu) return __int_as_float(0x7fc00000);
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+
+// One warp per token, lane l holding experts l, l + 32, ... (V of them). grid = ceil(T / kTokens).
+// table[b][e] receives block b's choices of expert e, all in the low and kept in the high 16 bits;
+// psum[b][e] the block's sum of P over kept tokens; row_stat[t] = (max logit, 1 / sum exp(l - max)),
+// the second 0 for tokens that are not kept.
+template <typename TL, int V>
+__global__ void __launch_bounds__(kThreads)
+    router_kernel(const TL* __restrict__ logits, const uint8_t* __restrict__ mask, int T, int E,
+                  int K, int32_t* __restrict__ ids, float* __restrict__ weights,
+                  float2* __restrict__ row_stat, uint32_t* __restrict__ table,
+                  float* __restrict__ psum) {
+  extern __shared__ uint32_t sm[];
+  uint32_t* hist = sm;                                    // [E]
+  float* wsum = reinterpret_cast<float*>(sm + E);         // [kWarps][E]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = threadIdx.x; e < E; e += kThreads) hist[e] = 0;
+  __syncthreads();
+  float acc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+  const int t0 = blockIdx.x * kTokens;
+  for (int t = t0 + warp; t < min(T, t0 + kTokens); t += kWarps) {
+    const TL* row = logits + static_cast<size_t>(t) * E;
+    float l[V];
+    uint32_t key[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int e = lane + 32 * i;
+      l[i] = e < E ? static_cast<float>(row[e]) : -INFINITY;
+      key[i] = e < E ? order_key(l[i]) : 0u;
+    }
+    float val = 0.f;  // lane j: the j-th choice
+    int id = 0;
+    for (int j = 0; j < K; ++j) {
+      uint32_t m = key[0];
+#pragma unroll
+      for (int i = 1; i < V; ++i) m = max(m, key[i]);
+      const uint32_t best = __reduce_max_sync(kAll, m);
+      int e_min = kMaxE;
+#pragma unroll
+      for (int i = V - 1; i >= 0; --i)
+        if (key[i] == best) e_min = lane + 32 * i;
+      const int chosen = __reduce_min_sync(kAll, e_min);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (lane + 32 * i == chosen) key[i] = 0u;
+      if (lane == j) {
+        val = key_value(best);
+        id = chosen;
+      }
+    }
+    const float top = __shfl_sync(kAll, val, 0);
+    const bool live = top != -INFINITY;
+    const bool kept = live && (mask == nullptr || mask[t] != 0);
+    // softmax over the choices, summed in choice order
+    const float ex = (lane < K && live) ? expf(val - top) : 0.f;
+    float s = 0.f;
+    for (int j = 0; j < K; ++j) s += __shfl_sync(kAll, ex, j);
+    const float inv_k = live ? 1.0f / s : 0.f;
+    if (lane < K) {
+      ids[static_cast<size_t>(t) * K + lane] = id;
+      weights[static_cast<size_t>(t) * K + lane] = ex * inv_k;
+      atomicAdd(&hist[id], kept ? 0x10001u : 1u);
+    }
+    // softmax over all experts
+    float inv = 0.f;
+    if (kept) {
+      float z = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        l[i] = expf(l[i] - top);
+        z += l[i];
+      }
+      inv = 1.0f / warp_sum(z);
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] = fmaf(l[i], inv, acc[i]);
+    }
+    if (lane == 0) row_stat[t] = make_float2(live ? top : 0.f, inv);
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (lane + 32 * i < E) wsum[warp * E + lane + 32 * i] = acc[i];
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += kThreads) {
+    float p = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) p += wsum[w * E + e];
+    psum[static_cast<size_t>(blockIdx.x) * E + e] = p;
+    table[static_cast<size_t>(blockIdx.x) * E + e] = hist[e];
+  }
+}
+
+// One cluster of up to 8 CTAs x 1024 threads; CTA r owns experts [r * CE, (r+1) * CE). Thread
+// (q, c) = (tid / CP, tid % CP), q < R, walks rows [q * per, (q+1) * per) of expert column c, so that
+// a warp reads 32 neighbouring experts. R is at most 32: one thread per expert adds the ranges up. Totals are exchanged through distributed shared memory.
+// Turns table into the dispatch's absolute start rows (in place, expert starts right behind it) and
+// writes the counts, the loss and coef[e] = E f_e / T' for the backward.
+__global__ void __launch_bounds__(1024)
+    router_finish_kernel(uint32_t* __restrict__ table, const float* __restrict__ psum, int nblocks,
+                         int E, int K, int CE, int CP, int64_t* __restrict__ tpe,
+                         int64_t* __restrict__ kept_counts, float* __restrict__ loss,
+                         float* __restrict__ coef) {
+  __shared__ int part_all[1024];     // [R][CP] range sums, then exclusive offsets of the ranges
+  __shared__ int part_kept[1024];
+  __shared__ double part_p[1024];
+  __shared__ int tot[kMaxE];         // every expert's totals (gathered from the whole cluster)
+  __shared__ int tot_kept[kMaxE];
+  __shared__ double tot_p[kMaxE];
+  __shared__ int start[kMaxE];
+  __shared__ double red[1024];
+  unsigned rank, ncta;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ncta));
+  const int tid = threadIdx.x;
+  const int R = min(1024 / CP, 32);
+  const int c = tid % CP, q = tid / CP;
+  const int e = static_cast<int>(rank) * CE + c;
+  const bool active = c < CE && e < E;
+  const int per = (nblocks + R - 1) / R;
+  const int b0 = min(nblocks, q * per), b1 = min(nblocks, b0 + per);
+  int all = 0, kept = 0;
+  double p = 0.0;
+  if (active) {
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) {
+      const uint32_t v = table[static_cast<size_t>(b) * E + e];
+      all += v & 0xffffu;
+      kept += v >> 16;
+      p += psum[static_cast<size_t>(b) * E + e];
+    }
+  }
+  part_all[tid] = all;
+  part_kept[tid] = kept;
+  part_p[tid] = p;
+  __syncthreads();
+  cluster_barrier();  // every CTA of the cluster runs before its shared memory is written
+  // totals of expert e (q == 0: this thread's own), scanned over its ranges, into every CTA
+  if (tid < CP && active) {
+    int run = 0, ksum = 0;
+    double ps = 0.0;
+    for (int j = 0; j < R; ++j) {
+      const int v = part_all[j * CP + c];
+      part_all[j * CP + c] = run;
+      run += v;
+      ksum += part_kept[j * CP + c];
+      ps += part_p[j * CP + c];
+    }
+    for (unsigned r = 0; r < ncta; ++r) {
+      uint32_t a, b, d;
+      const uint32_t la = static_cast<uint32_t>(__cvta_generic_to_shared(&tot[e]));
+      const uint32_t lb = static_cast<uint32_t>(__cvta_generic_to_shared(&tot_kept[e]));
+      const uint32_t ld = static_cast<uint32_t>(__cvta_generic_to_shared(&tot_p[e]));
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(la), "r"(r));
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(lb), "r"(r));
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(ld), "r"(r));
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(run) : "memory");
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(b), "r"(ksum) : "memory");
+      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(d), "d"(ps) : "memory");
+    }
+  }
+  cluster_barrier();
+  // exclusive scan of the totals over experts, and the sum of kept choices (every CTA alike)
+  start[tid] = tid < E ? tot[tid] : 0;
+  part_kept[tid] = tid < E ? tot_kept[tid] : 0;
+  __syncthreads();
+  for (int o = 1; o < E; o <<= 1) {
+    const int v = tid >= o ? start[tid - o] : 0;
+    const int k = tid >= o ? part_kept[tid - o] : 0;
+    __syncthreads();
+    start[tid] += v;
+    part_kept[tid] += k;
+    __syncthreads();
+  }
+  const long long choices = part_kept[E - 1];  // top_k T'
+  if (active) {
+    const int first = start[e] - tot[e];
+    if (q == 0) reinterpret_cast<int*>(table)[static_cast<size_t>(nblocks) * E + e] = first;
+    int run = first + part_all[tid];
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) {
+      const size_t i = static_cast<size_t>(b) * E + e;
+      const int v = table[i] & 0xffffu;
+      table[i] = static_cast<uint32_t>(run);
+      run += v;
+    }
+  }
+  if (rank == 0) {
+    const double kept_tokens = static_cast<double>(choices) / K;
+    double term = 0.0;
+    if (tid < E) {
+      tpe[tid] = tot[tid];
+      kept_counts[tid] = tot_kept[tid];
+      const double f = choices > 0 ? static_cast<double>(tot_kept[tid]) / choices : 0.0;
+      term = choices > 0 ? E * f * tot_p[tid] / kept_tokens : 0.0;
+      coef[tid] = choices > 0 ? static_cast<float>(E * f / kept_tokens) : 0.f;
+    }
+    red[tid] = term;
+    __syncthreads();
+    for (int o = 512; o > 0; o >>= 1) {
+      if (o >= E) continue;  // nothing but zeros behind E
+      if (tid < o) red[tid] += red[tid + o];
+      __syncthreads();
+    }
+    if (tid == 0) *loss = static_cast<float>(red[0]);
+  }
+}
+
+// One warp per token, persistent over tokens so that a lane's coefficients stay in registers. Every
+// warp owns E floats of shared memory in which the k choices' gradients are laid out by expert.
+template <typename TL, int V>
+__global__ void __launch_bounds__(kThreads)
+    router_backward_kernel(const TL* __restrict__ logits, const float2* __restrict__ row_stat,
+                           const int32_t* __restrict__ ids, const float* __restrict__ weights,
+                           const float* __restrict__ coef, const float* __restrict__ grad_w,
+                           const float* __restrict__ grad_loss, int T, int E, int K,
+                           TL* __restrict__ out) {
+  extern __shared__ uint32_t sm[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* add = reinterpret_cast<float*>(sm) + warp * E;
+  for (int e = lane; e < E; e += 32) add[e] = 0.f;
+  const float gl = grad_loss ? *grad_loss : 0.f;
+  float cf[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) cf[i] = lane + 32 * i < E ? gl * coef[lane + 32 * i] : 0.f;
+  __syncwarp();
+  for (int t = blockIdx.x * kWarps + warp; t < T; t += gridDim.x * kWarps) {
+    const TL* row = logits + static_cast<size_t>(t) * E;
+    const float2 st = row_stat[t];
+    float p[V];
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int e = lane + 32 * i;
+      p[i] = (e < E && st.y != 0.f) ? expf(static_cast<float>(row[e]) - st.x) * st.y : 0.f;
+      dot = fmaf(p[i], cf[i], dot);
+    }
+    dot = warp_sum(dot);
+    int id = 0;
+    if (grad_w) {
+      float w = 0.f, u = 0.f;
+      if (lane < K) {
+        id = ids[static_cast<size_t>(t) * K + lane];
+        w = weights[static_cast<size_t>(t) * K + lane];
+        u = grad_w[static_cast<size_t>(t) * K + lane];
+      }
+      const float mean = warp_sum(w * u);
+      if (lane < K) add[id] = w * (u - mean);
+      __syncwarp();
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int e = lane + 32 * i;
+      if (e < E)
+        out[static_cast<size_t>(t) * E + e] = static_cast<TL>(fmaf(p[i], cf[i] - dot, add[e]));
+    }
+    if (grad_w) {
+      __syncwarp();
+      if (lane < K) add[id] = 0.f;
+      __syncwarp();
+    }
+  }
+}
+
+int blocks_for(int64_t T) { return static_cast<int>((T + kTokens - 1) / kTokens); }
+
+template <typename TL, int V>
+int launch_router(const void* logits, const uint8_t* mask, int T, int E, int K, int32_t* ids,
+                  float* w, float2* stat, uint32_t* table, float* psum, cudaStream_t stream) {
+  const size_t smem = static_cast<size_t>(E) * (1 + kWarps) * 4;  // at most 36 KB
+  router_kernel<TL, V><<<blocks_for(T), kThreads, smem, stream>>>(
+      static_cast<const TL*>(logits), mask, T, E, K, ids, w, stat, table, psum);
+  return check_launch();
+}
+
+template <typename TL, int V>
+int launch_backward(const void* logits, const float2* stat, const int32_t* ids, const float* w,
+                    const float* coef, const float* gw, const float* gl, int T, int E, int K,
+                    void* out, cudaStream_t stream) {
+  const size_t smem = static_cast<size_t>(E) * kWarps * 4;
+  const int want = (T + kWarps - 1) / kWarps;
+  const int grid = want < 148 * 8 ? want : 148 * 8;
+  router_backward_kernel<TL, V><<<grid, kThreads, smem, stream>>>(
+      static_cast<const TL*>(logits), stat, ids, w, coef, gw, gl, T, E, K, static_cast<TL*>(out));
+  return check_launch();
+}
+
+// Calls f<TL, V>() with TL by dtype and V the smallest power of two that holds ceil(E / 32).
+#define GGO_ROUTER_CALL_V(TL, FN, ...)                          \
+  (E <= 32    ? FN<TL, 1>(__VA_ARGS__)                          \
+   : E <= 64  ? FN<TL, 2>(__VA_ARGS__)                          \
+   : E <= 128 ? FN<TL, 4>(__VA_ARGS__)                          \
+   : E <= 256 ? FN<TL, 8>(__VA_ARGS__)                          \
+   : E <= 512 ? FN<TL, 16>(__VA_ARGS__)                         \
+              : FN<TL, 32>(__VA_ARGS__))
+#define GGO_ROUTER_CALL(FN, ...)                                             \
+  (dtype == GGO_DTYPE_FP32   ? GGO_ROUTER_CALL_V(float, FN, __VA_ARGS__)     \
+   : dtype == GGO_DTYPE_BF16 ? GGO_ROUTER_CALL_V(__nv_bfloat16, FN, __VA_ARGS__) \
+                             : GGO_ROUTER_CALL_V(__half, FN, __VA_ARGS__))
+
+bool router_args_ok(int64_t num_tokens, int num_experts, int top_k) {
+  return num_tokens >= 0 && num_experts > 0 && num_experts <= kMaxE && top_k > 0 &&
+         top_k <= kMaxK && top_k <= num_experts;
+}
+
+bool router_dtype_ok(int dtype) {
+  return dtype == GGO_DTYPE_FP32 || dtype == GGO_DTYPE_BF16 || dtype == GGO_DTYPE_FP16;
+}
+
+}  // namespace
+}  // namespace ggo
+
+extern "C" {
+
+size_t ggo_moe_router_scratch_bytes(int64_t num_tokens, int num_experts) {
+  if (num_tokens < 0 || num_experts <= 0) return 16;
+  // the dispatch's table and expert starts (as ggo_moe_route_scratch_bytes), then the sums of P
+  return (2 * static_cast<size_t>(ggo::blocks_for(num_tokens)) + 1) * num_experts * 4;
+}
+
+int ggo_moe_router(const void* logits_dev, int dtype, int64_t num_tokens, int num_experts,
+                   int top_k, const uint8_t* token_mask_dev, int32_t* topk_ids_dev,
+                   float* topk_weights_dev, int64_t* tokens_per_expert_dev,
+                   int64_t* balance_counts_dev, float* balance_loss_dev, float* row_stat_dev,
+                   float* coef_dev, void* scratch_dev, cudaStream_t stream) {
+  if (!ggo::router_args_ok(num_tokens, num_experts, top_k)) return GGO_ERR_INVALID_ARG;
+  if (!tokens_per_expert_dev || !balance_counts_dev || !balance_loss_dev || !coef_dev ||
+      !scratch_dev)
+    return GGO_ERR_INVALID_ARG;
+  if (num_tokens > 0 && (!logits_dev || !topk_ids_dev || !topk_weights_dev || !row_stat_dev))
+    return GGO_ERR_INVALID_ARG;
+  if (!ggo::router_dtype_ok(dtype)) return GGO_ERR_DTYPE;
+  if (num_tokens * top_k > INT32_MAX) return GGO_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(row_stat_dev) & 7u) ||
+      (reinterpret_cast<uintptr_t>(scratch_dev) & 3u))
+    return GGO_ERR_ALIGNMENT;
+  const int T = static_cast<int>(num_tokens), E = num_experts;
+  const int nb = ggo::blocks_for(num_tokens);
+  uint32_t* table = static_cast<uint32_t*>(scratch_dev);
+  float* psum = reinterpret_cast<float*>(table + (static_cast<size_t>(nb) + 1) * E);
+  if (nb > 0) {
+    const int st = GGO_ROUTER_CALL(ggo::launch_router, logits_dev, token_mask_dev, T, E, top_k,
+                                   topk_ids_dev, topk_weights_dev,
+                                   reinterpret_cast<float2*>(row_stat_dev), table, psum, stream);
+    if (st) return st;
+  }
+  // experts per CTA: 32 (a coalesced row piece), or E / 8 beyond 256 experts
+  int ncta = 1;
+  while (ncta < 8 && ncta * 32 < E) ncta *= 2;
+  const int CE = (E + ncta - 1) / ncta;
+  int CP = 1;
+  while (CP < CE) CP *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ncta, 1, 1);
+  cfg.blockDim = dim3(1024, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ncta;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, ggo::router_finish_kernel, table,
+                                         static_cast<const float*>(psum), nb, E, top_k, CE, CP,
+                                         tokens_per_expert_dev, balance_counts_dev,
+                                         balance_loss_dev, coef_dev))
+    return ggo::cuda_fail(static_cast<int>(e));
+  return ggo::check_launch();
+}
+
+int ggo_moe_router_backward(const void* logits_dev, int dtype, int64_t num_tokens, int num_experts,
+                            int top_k, const int32_t* topk_ids_dev, const float* topk_weights_dev,
+                            const float* row_stat_dev, const float* coef_dev,
+                            const float* grad_weights_dev, const float* grad_loss_dev,
+                            void* grad_logits_dev, cudaStream_t stream) {
+  if (!ggo::router_args_ok(num_tokens, num_experts, top_k)) return GGO_ERR_INVALID_ARG;
+  if (!ggo::router_dtype_ok(dtype)) return GGO_ERR_DTYPE;
+  if (num_tokens * top_k > INT32_MAX) return GGO_ERR_SHAPE;
+  if (num_tokens == 0) return GGO_OK;
+  if (!logits_dev || !topk_ids_dev || !topk_weights_dev || !row_stat_dev || !coef_dev ||
+      !grad_logits_dev)
+    return GGO_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(row_stat_dev) & 7u) return GGO_ERR_ALIGNMENT;
+  const int T = static_cast<int>(num_tokens), E = num_experts;
+  return GGO_ROUTER_CALL(ggo::launch_backward, logits_dev,
+                         reinterpret_cast<const float2*>(row_stat_dev), topk_ids_dev,
+                         topk_weights_dev, coef_dev, grad_weights_dev, grad_loss_dev, T, E, top_k,
+                         grad_logits_dev, stream);
+}
+
+}  // extern "C"

@@ -72,6 +72,26 @@ void* workspace_for(const torch::Device& dev, cudaStream_t stream) {
   return it->second.data_ptr();
 }
 
+// Workspace of one call. Eager calls share the stream's workspace (they run in stream order). A
+// captured call gets a zero-filled one of its own inside the graph, so that replays of several
+// graphs may overlap each other and eager calls; its device errors still go to the stream's.
+struct CallWorkspace {
+  torch::Tensor own;  // captured calls only
+  void* ws = nullptr;
+  int* err = nullptr;
+
+  CallWorkspace(const torch::Device& dev, cudaStream_t stream) {
+    void* shared = workspace_for(dev, stream);
+    ws = shared;
+    err = ggo_workspace_error_word(shared);
+    if (capturing(stream)) {
+      own = torch::zeros({static_cast<int64_t>(ggo_workspace_size())},
+                         torch::TensorOptions().dtype(torch::kUInt8).device(dev));
+      ws = own.data_ptr();
+    }
+  }
+};
+
 torch::Tensor counts_on_device(const torch::Tensor& counts, const torch::Device& dev) {
   auto c = counts.to(torch::kInt64);
   if (!c.is_cuda() || c.device() != dev) c = c.to(dev, /*non_blocking=*/true);
@@ -348,6 +368,177 @@ torch::Tensor grouped_gemm_swiglu(const torch::Tensor& x, const torch::Tensor& w
       sort_by_m ? 1 : 0, workspace_for(x.device(), stream), stream);
   check_status(st, "gate/up SwiGLU grouped GEMM");
   return h;
+}
+
+// ------------------------------------------------------------------ INT8
+// Row-wise INT8 quantisation: returns (q int8, same shape, scale fp32 without the last dimension).
+std::tuple<torch::Tensor, torch::Tensor> quantize_int8_rows(const torch::Tensor& x) {
+  TORCH_CHECK(x.is_cuda() && x.is_contiguous() && x.dim() >= 2, "x must be contiguous CUDA");
+  TORCH_CHECK(x.size(-1) > 0, "x must have columns");
+  c10::cuda::CUDAGuard guard(x.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const int64_t cols = x.size(-1), rows = x.numel() / cols;
+  auto q = torch::empty(x.sizes(), x.options().dtype(torch::kInt8));
+  auto sizes = x.sizes().vec();
+  sizes.pop_back();
+  auto s = torch::empty(sizes, x.options().dtype(torch::kFloat32));
+  check_status(ggo_quantize_int8_rows(x.data_ptr(), rows, cols, dtype_code(x), q.data_ptr(),
+                                      s.data_ptr<float>(), stream),
+               "int8 quantisation");
+  return {q, s};
+}
+
+// Token counts of an INT8 call on `dev`: device counts as they are, host counts copied before the
+// call returns (never inside a capture, which would replay the copy from freed host memory).
+torch::Tensor counts_for_call(const torch::Tensor& counts, const torch::Device& dev,
+                              cudaStream_t stream) {
+  TORCH_CHECK(counts.dim() == 1, "token counts must be 1D");
+  TORCH_CHECK(counts.is_cuda() || !capturing(stream),
+              "token counts must be on the GPU while a CUDA graph is captured");
+  TORCH_CHECK(!counts.is_cuda() || counts.device() == dev, "token counts on another device");
+  return counts.to(torch::TensorOptions().dtype(torch::kInt64).device(dev)).contiguous();
+}
+
+// INT8 grouped GEMM (swiglu: weights [E, 2F, K], result [T, F]), result bf16 or fp16.
+torch::Tensor grouped_gemm_int8(const torch::Tensor& a_q, const torch::Tensor& a_scale,
+                                const torch::Tensor& w_q, const torch::Tensor& w_scale,
+                                const torch::Tensor& counts, bool swiglu, torch::Dtype out_dtype,
+                                int64_t tile_config, bool sort_by_m) {
+  TORCH_CHECK(a_q.is_cuda() && w_q.is_cuda() && a_q.dim() == 2 && w_q.dim() == 3,
+              "a_q [T, K] and w_q [E, N, K] CUDA tensors");
+  TORCH_CHECK(a_q.scalar_type() == torch::kInt8 && w_q.scalar_type() == torch::kInt8,
+              "operands must be int8");
+  TORCH_CHECK(a_q.size(1) == w_q.size(2), "K mismatch: input=", a_q.size(1), " vs weights=",
+              w_q.size(2));
+  TORCH_CHECK(a_q.is_contiguous() && w_q.is_contiguous(), "operands must be contiguous");
+  TORCH_CHECK(a_scale.scalar_type() == torch::kFloat32 && a_scale.dim() == 1 &&
+                  a_scale.size(0) == a_q.size(0) && a_scale.is_contiguous(),
+              "input_scale must be contiguous fp32 [T]");
+  TORCH_CHECK(w_scale.scalar_type() == torch::kFloat32 && w_scale.dim() == 2 &&
+                  w_scale.size(0) == w_q.size(0) && w_scale.size(1) == w_q.size(1) &&
+                  w_scale.is_contiguous(),
+              "weight_scale must be contiguous fp32 [E, N]");
+  for (const auto& t : {a_scale, w_q, w_scale})
+    TORCH_CHECK(t.device() == a_q.device(), "operands and scales on different devices");
+  TORCH_CHECK(!swiglu || w_q.size(1) % 2 == 0, "w_gate_up must have 2F rows per expert");
+  TORCH_CHECK(counts.numel() == w_q.size(0), "tokens_per_expert must have num_experts entries");
+  TORCH_CHECK(out_dtype == torch::kBFloat16 || out_dtype == torch::kHalf,
+              "Unsupported dtype: ", out_dtype);
+  c10::cuda::CUDAGuard guard(a_q.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const int64_t T = a_q.size(0), K = a_q.size(1), E = w_q.size(0);
+  const int64_t N = swiglu ? w_q.size(1) / 2 : w_q.size(1);
+  auto out = torch::empty({T, N}, a_q.options().dtype(out_dtype));
+  if (T == 0) return out;
+  auto c = counts_for_call(counts, a_q.device(), stream);
+  CallWorkspace ws(a_q.device(), stream);
+  const int st = ggo_grouped_gemm_int8(
+      a_q.data_ptr(), a_scale.data_ptr<float>(), w_q.data_ptr(), w_scale.data_ptr<float>(),
+      out.data_ptr(), c.data_ptr<int64_t>(), static_cast<int>(E), static_cast<int>(E), T, N, K,
+      dtype_code(out), swiglu ? 1 : 0, static_cast<int>(tile_config), sort_by_m ? 1 : 0, ws.ws,
+      ws.err, stream);
+  check_status(st, swiglu ? "int8 gate/up SwiGLU grouped GEMM" : "int8 grouped GEMM");
+  return out;
+}
+
+// ------------------------------------------------------------------ router with balance loss
+int logits_dtype(const torch::Tensor& t) {
+  if (t.scalar_type() == torch::kFloat32) return GGO_DTYPE_FP32;
+  return dtype_code(t);
+}
+
+// Returns (topk_ids, topk_weights, tokens_per_expert, balance_loss, balance_counts, scratch,
+// row_stat, coef); the last two are what moe_router_backward takes.
+std::vector<torch::Tensor> moe_router(const torch::Tensor& logits, int64_t top_k,
+                                      const c10::optional<torch::Tensor>& mask) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.is_contiguous(),
+              "router_logits must be a contiguous 2D CUDA tensor");
+  const int64_t T = logits.size(0), E = logits.size(1);
+  TORCH_CHECK(E <= INT32_MAX && top_k > 0 && top_k <= E, "top_k must be in [1, num_experts]");
+  const uint8_t* mp = nullptr;
+  if (mask.has_value()) {
+    TORCH_CHECK(mask->device() == logits.device() && mask->scalar_type() == torch::kBool &&
+                    mask->dim() == 1 && mask->size(0) == T && mask->is_contiguous(),
+                "token_mask must be a contiguous bool tensor [T] on the logits' device");
+    mp = reinterpret_cast<const uint8_t*>(mask->data_ptr<bool>());
+  }
+  c10::cuda::CUDAGuard guard(logits.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const auto f32 = torch::TensorOptions().dtype(torch::kFloat32).device(logits.device());
+  const auto i32 = f32.dtype(torch::kInt32), i64 = f32.dtype(torch::kInt64);
+  auto ids = torch::empty({T, top_k}, i32);
+  auto w = torch::empty({T, top_k}, f32);
+  auto tpe = torch::empty({E}, i64), kept = torch::empty({E}, i64);
+  auto loss = torch::empty({}, f32), coef = torch::empty({E}, f32);
+  auto stat = torch::empty({T, 2}, f32);
+  const size_t sb = ggo_moe_router_scratch_bytes(T, static_cast<int>(E));
+  auto scratch = torch::empty({static_cast<int64_t>((sb + 3) / 4)}, i32);
+  check_status(ggo_moe_router(logits.data_ptr(), logits_dtype(logits), T, static_cast<int>(E),
+                              static_cast<int>(top_k), mp, ids.data_ptr<int32_t>(),
+                              w.data_ptr<float>(), tpe.data_ptr<int64_t>(),
+                              kept.data_ptr<int64_t>(), loss.data_ptr<float>(),
+                              stat.data_ptr<float>(), coef.data_ptr<float>(), scratch.data_ptr(),
+                              stream),
+               "MoE router");
+  return {ids, w, tpe, loss, kept, scratch, stat, coef};
+}
+
+torch::Tensor moe_router_backward(const torch::Tensor& logits, const torch::Tensor& ids,
+                                  const torch::Tensor& w, const torch::Tensor& stat,
+                                  const torch::Tensor& coef,
+                                  const c10::optional<torch::Tensor>& grad_w,
+                                  const c10::optional<torch::Tensor>& grad_loss) {
+  const float *gw = nullptr, *gl = nullptr;
+  if (grad_w.has_value()) {
+    TORCH_CHECK(grad_w->sizes() == w.sizes() && grad_w->scalar_type() == torch::kFloat32 &&
+                    grad_w->is_contiguous() && grad_w->device() == logits.device(),
+                "gradient of the weights: contiguous fp32 [T, top_k]");
+    gw = grad_w->data_ptr<float>();
+  }
+  if (grad_loss.has_value()) {
+    TORCH_CHECK(grad_loss->numel() == 1 && grad_loss->scalar_type() == torch::kFloat32 &&
+                    grad_loss->device() == logits.device(),
+                "gradient of the balance loss: one fp32");
+    gl = grad_loss->data_ptr<float>();
+  }
+  c10::cuda::CUDAGuard guard(logits.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  auto out = torch::empty_like(logits);
+  check_status(ggo_moe_router_backward(
+                   logits.data_ptr(), logits_dtype(logits), logits.size(0),
+                   static_cast<int>(logits.size(1)), static_cast<int>(ids.size(1)),
+                   ids.data_ptr<int32_t>(), w.data_ptr<float>(), stat.data_ptr<float>(),
+                   coef.data_ptr<float>(), gw, gl, out.data_ptr(), stream),
+               "MoE router backward");
+  return out;
+}
+
+// Permute with INT8 quantisation: returns (q_sorted int8 [T*k, H], scale fp32 [T*k], slot_pos int32).
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_permute_int8(
+    const torch::Tensor& x, const torch::Tensor& topk_ids, const torch::Tensor& scratch,
+    int64_t num_experts) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous(), "hidden must be 2D contiguous CUDA");
+  TORCH_CHECK(topk_ids.scalar_type() == torch::kInt32 && topk_ids.is_contiguous() &&
+                  topk_ids.dim() == 2 && topk_ids.size(0) == x.size(0) &&
+                  topk_ids.device() == x.device(),
+              "topk_ids must be contiguous int32 [T, top_k] on hidden's device");
+  const int64_t T = x.size(0), H = x.size(1), k = topk_ids.size(1);
+  TORCH_CHECK(num_experts > 0 && num_experts <= INT32_MAX &&
+                  scratch.scalar_type() == torch::kInt32 && scratch.device() == x.device() &&
+                  static_cast<size_t>(scratch.numel()) * 4 >=
+                      ggo_moe_route_scratch_bytes(T, static_cast<int>(num_experts)),
+              "scratch must be the router's");
+  c10::cuda::CUDAGuard guard(x.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  auto q = torch::empty({T * k, H}, x.options().dtype(torch::kInt8));
+  auto s = torch::empty({T * k}, x.options().dtype(torch::kFloat32));
+  auto spos = torch::empty({T * k}, x.options().dtype(torch::kInt32));
+  check_status(ggo_moe_permute_int8(x.data_ptr(), T, H, static_cast<int>(num_experts),
+                                    static_cast<int>(k), topk_ids.data_ptr<int32_t>(),
+                                    q.data_ptr(), s.data_ptr<float>(), spos.data_ptr<int32_t>(),
+                                    scratch.data_ptr(), dtype_code(x), stream),
+               "MoE permute with int8 quantisation");
+  return {q, s, spos};
 }
 
 // Router: returns (topk_ids int32 [T,k], topk_weights fp32 [T,k], tokens_per_expert int64 [E],
@@ -697,6 +888,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("tile_config") = 4, py::arg("sort_by_m") = true);
   m.def("grouped_gemm_swiglu", &grouped_gemm_swiglu, py::arg("x"), py::arg("w_gate_up"),
         py::arg("tokens_per_segment"), py::arg("num_experts"), py::arg("sort_by_m") = true);
+  m.def("quantize_int8_rows", &quantize_int8_rows, py::arg("x"));
+  m.def("grouped_gemm_int8", &grouped_gemm_int8, py::arg("input_q"), py::arg("input_scale"),
+        py::arg("weights_q"), py::arg("weight_scale"), py::arg("tokens_per_expert"),
+        py::arg("swiglu"), py::arg("out_dtype"),
+        py::arg("tile_config") = 4, py::arg("sort_by_m") = true);
+  m.def("moe_router", &moe_router, py::arg("router_logits"), py::arg("top_k"),
+        py::arg("token_mask") = py::none());
+  m.def("moe_router_backward", &moe_router_backward, py::arg("router_logits"), py::arg("topk_ids"),
+        py::arg("topk_weights"), py::arg("row_stat"), py::arg("coef"), py::arg("grad_weights"),
+        py::arg("grad_loss"));
+  m.def("moe_permute_int8", &moe_permute_int8, py::arg("hidden"), py::arg("topk_ids"),
+        py::arg("scratch"), py::arg("num_experts"));
   m.def("moe_route", &moe_route, py::arg("router_logits"), py::arg("top_k"));
   m.def("moe_permute", &moe_permute, py::arg("hidden"), py::arg("topk_ids"), py::arg("scratch"),
         py::arg("num_experts"));

@@ -31,6 +31,7 @@ from typing import Callable, Optional
 
 import torch
 import torch.distributed as dist
+from torch.autograd.function import once_differentiable
 
 from grouped_gemm_opt.ops import TileConfig
 
@@ -91,6 +92,88 @@ def cuda_ops() -> MoEOps:
         down=lambda h, w, c, e, s: _C.grouped_gemm_segments(h, w, c, e, int(TileConfig.AUTO), s),
         combine=lambda y, w, pos: _C.moe_combine(y, w, pos),
     )
+
+
+@dataclass
+class MoERouting:
+    """What :func:`moe_router` returns: the routing of T tokens over E experts, for the caller and
+    (``fused_moe(..., routing=...)``) for the layers."""
+    topk_ids: torch.Tensor           # [T, top_k] int32, in descending-logit order
+    topk_weights: torch.Tensor       # [T, top_k] fp32, differentiable
+    tokens_per_expert: torch.Tensor  # [E] int64, choices of all tokens (what the GEMMs take)
+    balance_loss: torch.Tensor       # fp32 scalar, differentiable
+    balance_counts: torch.Tensor     # [E] int64, choices of the tokens the loss is over
+    scratch: torch.Tensor            # the dispatch's offset table
+
+
+class _RouterFn(torch.autograd.Function):
+    """Forward: the routing kernel with the balance loss; backward: one kernel for the gradients that
+    reach the logits through the weights and through the loss."""
+
+    @staticmethod
+    def forward(ctx, logits, top_k, mask):
+        from grouped_gemm_opt._native import _C
+        ids, w, tpe, loss, kept, scratch, stat, coef = _C.moe_router(logits, top_k, mask)
+        ctx.save_for_backward(logits, ids, w, stat, coef)
+        ctx.mark_non_differentiable(ids, tpe, kept, scratch)
+        ctx.set_materialize_grads(False)
+        return ids, w, tpe, loss, kept, scratch
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _ids, grad_w, _tpe, grad_loss, _kept, _scratch):
+        from grouped_gemm_opt._native import _C
+        if grad_w is None and grad_loss is None:
+            return None, None, None
+        logits, ids, w, stat, coef = ctx.saved_tensors
+        if grad_w is not None:
+            grad_w = grad_w.contiguous()
+        return (_C.moe_router_backward(logits, ids, w, stat, coef, grad_w, grad_loss), None, None)
+
+
+def moe_router(router_logits: torch.Tensor, top_k: int,
+               token_mask: Optional[torch.Tensor] = None) -> MoERouting:
+    """Top-k routing with the load-balance loss and per-expert counts, differentiable.
+
+    The routing is the layers' own (top-k of the fp32 logits, ties to the lower index, softmax over
+    the chosen ones). Over the kept tokens, with ``f_e`` the share of their choices that fell on
+    expert e and ``p_e`` the mean over them of the softmax over ALL experts::
+
+        balance_loss = E * sum_e f_e * p_e          # 1 when balanced
+
+    The loss's gradient reaches the logits through p, that of ``topk_weights`` through the chosen
+    logits; one kernel computes both.
+
+    Args:
+        router_logits: [T, E] fp32, bf16 or fp16 on the GPU, E <= 1024.
+        top_k: experts per token, 1..min(16, E).
+        token_mask: [T] bool, False for padding. A masked token is routed like any other (its rows
+            keep their place in static shapes) and counts in ``tokens_per_expert``; it takes no part
+            in the loss, its gradient or ``balance_counts``. A token whose logits are all -inf
+            has weights 0 and is not kept either. Without kept tokens the loss is 0.
+
+    Nothing synchronises; equal inputs give equal bits. Can be captured in a CUDA graph, the backward
+    together with the forward.
+    """
+    assert router_logits.is_cuda and router_logits.dim() == 2
+    assert 0 < top_k <= router_logits.size(1)
+    if token_mask is not None:
+        assert token_mask.dim() == 1 and token_mask.size(0) == router_logits.size(0), (
+            "token_mask must have one entry per token")
+        token_mask = token_mask.contiguous()
+    return MoERouting(*_RouterFn.apply(router_logits.contiguous(), top_k, token_mask))
+
+
+def _routing_of(routing: MoERouting, router_logits, top_k):
+    """The stage outputs (ids, weights, tokens_per_expert, scratch) of a given routing, after checks
+    that it belongs to these logits' shape and device."""
+    T, E = router_logits.shape
+    assert routing.topk_ids.shape == (T, top_k) and routing.tokens_per_expert.shape == (E,), (
+        f"routing is for {tuple(routing.topk_ids.shape)} choices over "
+        f"{routing.tokens_per_expert.numel()} experts, the layer for {(T, top_k)} over {E}")
+    assert routing.topk_ids.device == router_logits.device, "routing on another device"
+    return (routing.topk_ids, routing.topk_weights.detach(), routing.tokens_per_expert,
+            routing.scratch)
 
 
 class EPBuffers:
@@ -183,7 +266,7 @@ class EPBuffers:
 
 
 def _fused_moe_p2p(hidden, router_logits, w_gate_up, w_down, top_k, bufs: "EPBuffers",
-                   sort_by_m, timer=None):
+                   sort_by_m, timer=None, routing=None):
     """Expert-parallel layer over NVLink peer memory: the dispatch kernel writes rows into the
     owners' receive buffers, the down GEMM's epilogue writes results back into the sources'
     return buffers. The phases are ordered by device-side epoch flags in the IPC-shared sync
@@ -199,7 +282,8 @@ def _fused_moe_p2p(hidden, router_logits, w_gate_up, w_down, top_k, bufs: "EPBuf
     bufs.epoch += 1
     ep, dev, boards, own = bufs.epoch, hidden.device.index, bufs.ptrs["board"], bufs._own["board"]
     lim = bufs.wait_limit_cycles
-    ids, w, tpe, scratch = C.moe_route(router_logits, top_k)
+    ids, w, tpe, scratch = (C.moe_route(router_logits, top_k) if routing is None
+                            else _routing_of(routing, router_logits, top_k))
     _mark(timer, "route")
     # phase 0: every rank's counts land in every board
     C.ep_publish_counts(tpe, boards, rank, 0, ep)
@@ -258,6 +342,7 @@ def fused_moe(
     ops: Optional[MoEOps] = None,
     ep_buffers: Optional[EPBuffers] = None,
     timer: Optional[StageEvents] = None,
+    routing: Optional[MoERouting] = None,
 ) -> torch.Tensor:
     """MoE layer forward.
 
@@ -273,6 +358,8 @@ def fused_moe(
         ep_buffers: EPBuffers of `ep_group`: selects the fused peer-memory path (dispatch and
             result scatter over NVLink inside the kernels) instead of NCCL all-to-alls.
         timer: a StageEvents that records a CUDA event after every stage (device timing).
+        routing: the result of ``moe_router(router_logits, top_k)``: the layer uses it instead of
+            routing again.
 
     Returns: [T, H] = sum_j w[t,j] * down(silu(gate(x_t)) * up(x_t)) for the top-k experts.
     """
@@ -282,11 +369,12 @@ def fused_moe(
         timer.start()
     if ep_buffers is not None and world > 1 and ops is None:
         return _fused_moe_p2p(hidden.contiguous(), router_logits, w_gate_up, w_down, top_k,
-                              ep_buffers, sort_by_m, timer)
+                              ep_buffers, sort_by_m, timer, routing)
     if ops is None:
         ops = cuda_ops()
     hidden = hidden.contiguous()
-    ids, w, tpe, scratch = ops.route(router_logits, top_k)
+    ids, w, tpe, scratch = (ops.route(router_logits, top_k) if routing is None
+                            else _routing_of(routing, router_logits, top_k))
     _mark(timer, "route")
     xs, _sorted_token, slot_pos = ops.permute(hidden, ids, scratch, E)
     _mark(timer, "dispatch")
@@ -537,3 +625,54 @@ def fused_moe_mxfp8(hidden: torch.Tensor, router_logits: torch.Tensor, weights: 
     _mark(timer, "combine")
     return out
 
+
+
+@dataclass
+class MoEInt8Weights:
+    """INT8 expert weights with one fp32 scale per output channel (see quantize_moe_weights_int8)."""
+    w_gate_up_q: torch.Tensor      # [E, 2F, H] int8
+    w_gate_up_scale: torch.Tensor  # [E, 2F] fp32
+    w_down_q: torch.Tensor         # [E, H, F] int8
+    w_down_scale: torch.Tensor     # [E, H] fp32
+
+
+def quantize_moe_weights_int8(w_gate_up: torch.Tensor, w_down: torch.Tensor) -> MoEInt8Weights:
+    """Per-output-channel INT8 quantisation of the layer's weights (done once, on the GPU)."""
+    from grouped_gemm_opt.ops import quantize_int8
+    gq, gs = quantize_int8(w_gate_up)
+    dq, ds = quantize_int8(w_down)
+    return MoEInt8Weights(gq, gs, dq, ds)
+
+
+def fused_moe_int8(hidden: torch.Tensor, router_logits: torch.Tensor, weights: MoEInt8Weights,
+                   top_k: int, sort_by_m: bool = True, timer: Optional[StageEvents] = None,
+                   routing: Optional[MoERouting] = None) -> torch.Tensor:
+    """Single-GPU MoE layer with INT8 grouped GEMMs: route -> dispatch, which quantises every token's
+    row once and gathers its codes -> gate/up GEMM with a scaled SwiGLU epilogue -> per-row
+    quantisation of h -> down GEMM with a scaled epilogue -> combine. h and the experts' results are
+    of hidden's type (bf16 or fp16), and so is the returned [T, H]. ``routing`` as in
+    :func:`fused_moe`. H and F multiples of 16. Not differentiable."""
+    assert hidden.is_cuda
+    T, H, E, _ = _check(hidden, router_logits, weights.w_gate_up_q, weights.w_down_q, top_k, 1)
+    if T == 0:
+        return torch.empty_like(hidden)
+    from grouped_gemm_opt._native import _C
+    if timer is not None:
+        timer.start()
+    ids, w, tpe, scratch = (_C.moe_route(router_logits, top_k) if routing is None
+                            else _routing_of(routing, router_logits, top_k))
+    _mark(timer, "route")
+    xq, xsc, slot_pos = _C.moe_permute_int8(hidden.contiguous(), ids, scratch, E)
+    _mark(timer, "dispatch")
+    tile = int(TileConfig.AUTO)
+    h = _C.grouped_gemm_int8(xq, xsc, weights.w_gate_up_q, weights.w_gate_up_scale, tpe, True,
+                             hidden.dtype, tile, sort_by_m)
+    _mark(timer, "gate_up")
+    hq, hsc = _C.quantize_int8_rows(h)
+    _mark(timer, "quantize_h")
+    y = _C.grouped_gemm_int8(hq, hsc, weights.w_down_q, weights.w_down_scale, tpe, False,
+                             hidden.dtype, tile, sort_by_m)
+    _mark(timer, "down")
+    out = _C.moe_combine(y, w, slot_pos)
+    _mark(timer, "combine")
+    return out

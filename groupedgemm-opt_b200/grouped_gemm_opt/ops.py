@@ -169,6 +169,45 @@ def grouped_gemm_opt_fp8(
                                tokens_per_expert, int(tile_config), sort_by_m)
 
 
+def quantize_int8(x: torch.Tensor):
+    """Row-wise INT8 quantisation on the GPU of a bf16/fp16 tensor: returns (q int8, scale fp32) with
+    x ~= q * scale[..., None]; scale = rowwise max|x| / 127 and q = 127 x / max|x| rounded half to
+    even, in [-127, 127] (computed exactly). Weights [E, N, K] quantise per output channel (scale
+    [E, N]). A zero row gets scale 1; a row with an infinity or NaN gets codes 0 and scale NaN, which
+    makes its products NaN. The last dimension must be a multiple of 16. Not differentiable."""
+    return _C.quantize_int8_rows(x.contiguous())
+
+
+def grouped_gemm_opt_int8(
+    input_q: torch.Tensor,
+    input_scale: torch.Tensor,
+    weights_q: torch.Tensor,
+    weight_scale: torch.Tensor,
+    tokens_per_expert: torch.Tensor,
+    tile_config: TileConfig = TileConfig.AUTO,
+    sort_by_m: bool = True,
+    out_dtype: torch.dtype = torch.bfloat16,
+) -> torch.Tensor:
+    """INT8 grouped GEMM: ``out[i] = (q_in[i] @ q_w[e(i)].T) * input_scale[i] * weight_scale[e(i)]``
+    with signed 8-bit operands, exact 32-bit integer sums (tcgen05 kind::i8) and a bf16 or fp16
+    result (``out_dtype``), rounded once. Use :func:`quantize_int8` to produce the operands and
+    scales; one expert (``weights_q`` [1, N, K]) makes it a plain linear layer.
+
+    K a multiple of 16, at most 131056 (a longer sum could leave 32 bits); N a multiple of 8. Counts
+    as in :func:`grouped_gemm_opt`; inside a CUDA-graph capture they must be on the GPU. Not
+    differentiable."""
+    assert input_q.is_cuda and weights_q.is_cuda
+    assert input_q.dim() == 2 and weights_q.dim() == 3
+    tokens_per_expert = tokens_per_expert.to(torch.int64).contiguous()
+    if not tokens_per_expert.is_cuda:
+        total = int(tokens_per_expert.sum().item())
+        assert total == input_q.size(0), (
+            f"sum(tokens_per_expert)={total} != total_tokens={input_q.size(0)}")
+    return _C.grouped_gemm_int8(input_q.contiguous(), input_scale.contiguous().float(),
+                                weights_q.contiguous(), weight_scale.contiguous().float(),
+                                tokens_per_expert, False, out_dtype, int(tile_config), sort_by_m)
+
+
 def quantize_mxfp8(x: torch.Tensor, tokens_per_expert: torch.Tensor = None):
     """MX e4m3 quantisation on the GPU in the OCP microscaling layout: every 32 consecutive
     elements of a row share one UE8M0 scale 2^(byte - 127). The scale rule is non-saturating

@@ -40,6 +40,7 @@ extern "C" {
 
 #define GGO_DTYPE_BF16 0
 #define GGO_DTYPE_FP16 1
+#define GGO_DTYPE_FP32 2 /* router logits only */
 
 #define GGO_MAX_SEGMENTS 1024
 #define GGO_WORKSPACE_BYTES 256
@@ -157,6 +158,36 @@ int ggo_grouped_gemm_swiglu_fp8(const void* x_dev, const float* x_scale_dev,
 int ggo_quantize_fp8_rows(const void* x_dev, int64_t rows, int64_t cols, int dtype, void* q_dev,
                           float* scale_dev, cudaStream_t stream);
 
+/* INT8 (no reference counterpart). Row-wise quantisation of a bf16/fp16 matrix [rows, cols] to signed
+ * 8-bit codes: scale_dev[r] = max|x[r,:]| / 127, q_dev[r,c] = 127 x[r,c] / max|x[r,:]| rounded half
+ * to even (exactly: the result is that of exact arithmetic), in [-127, 127]. A zero row gets scale 1.
+ * A row that holds an infinity or a NaN gets scale NaN and codes 0, so every product with it is NaN.
+ * Weights [E, N, K] quantise per output channel as rows = E*N. cols a multiple of 16. */
+int ggo_quantize_int8_rows(const void* x_dev, int64_t rows, int64_t cols, int dtype, void* q_dev,
+                           float* scale_dev, cudaStream_t stream);
+
+/* INT8 grouped GEMM with one scale per row and per output channel:
+ *   out[r, n] = (sum_k a[r,k] * b[e(r),n,k]) * input_scale[r] * weight_scale[e(r), n]
+ * input_dev [T, K] and weights_dev [E, N, K] signed bytes, the sums exact 32-bit integers
+ * (tcgen05 kind::i8), the two products with the scales in fp32, rounded once to out_dtype (bf16 or
+ * fp16). swiglu != 0: weights_dev [E, 2N, K] holds N gate rows then N up rows, weight_scale_dev
+ * [E, 2N], and out[r, n] = silu(gate) * up (N = F). Segment semantics as
+ * ggo_grouped_gemm_segments. K a multiple of 16 and at most GGO_INT8_MAX_K (beyond it a sum of products
+ * could leave 32 bits: GGO_ERR_SHAPE), N of 8. error_dev: a device word that receives device errors
+ * (see ggo_workspace_error), or NULL for the workspace's own; with it a call can have a workspace
+ * of its own (a captured graph that may be replayed beside other work) and still report where the
+ * caller looks. */
+#define GGO_INT8_MAX_K 131056
+int ggo_grouped_gemm_int8(const void* input_dev, const float* input_scale_dev,
+                          const void* weights_dev, const float* weight_scale_dev,
+                          void* output_dev, const int64_t* tokens_per_segment_dev,
+                          int num_segments, int num_experts, int64_t total_tokens, int64_t N,
+                          int64_t K, int out_dtype, int swiglu, int tile_config, int sort_by_m,
+                          void* workspace_dev, int* error_dev, cudaStream_t stream);
+
+/* Address of a workspace's device error word (what ggo_workspace_error reads), for error_dev. */
+int* ggo_workspace_error_word(void* workspace_dev);
+
 /* MXFP8: block-scaled e4m3 in the OCP MX layout (no reference counterpart). Every 32 consecutive
  * K elements of a row share one UE8M0 scale 2^(byte - 127); the tensor cores apply both operands'
  * scales (tcgen05 kind::mxf8f6f4.block_scale) and accumulate in fp32. The GEMMs accept any UE8M0
@@ -227,6 +258,43 @@ size_t ggo_moe_route_scratch_bytes(int64_t num_tokens, int num_experts);
 int ggo_moe_route(const float* logits_dev, int64_t num_tokens, int num_experts, int top_k,
                   int32_t* topk_ids_dev, float* topk_weights_dev,
                   int64_t* tokens_per_expert_dev, void* scratch_dev, cudaStream_t stream);
+
+/* Router with balance loss (no reference counterpart). Routing as ggo_moe_route (equal ids and
+ * weights), reading logits of any of the three dtypes, and over the kept tokens -- token_mask_dev[t]
+ * != 0 (NULL: all) and a logit above -inf -- the balance loss
+ *   E * sum_e f_e p_e,  f_e = share of the kept tokens' choices that fell on e,  p_e = mean softmax
+ * (over all E logits) probability of e: 1 when balanced, 0 when no token is kept. Masked tokens are
+ * routed like the others and count in tokens_per_expert_dev [E] (what the grouped GEMMs take);
+ * balance_counts_dev [E] holds the kept tokens' choices. A token whose logits are all -inf gets the
+ * weights 0. Signed zeros tie; NaN ranks above +inf and makes its token's weights and the loss NaN.
+ * For the backward: row_stat_dev [T, 2] fp32 (8-byte aligned), coef_dev [E] fp32.
+ * scratch_dev: ggo_moe_router_scratch_bytes(T, E) bytes; its head is what ggo_moe_permute,
+ * ggo_ep_dispatch and ggo_moe_permute_int8 take. Sums are taken in a fixed order: equal inputs give
+ * equal bits. E <= 1024, top_k <= 16, top_k <= E. */
+size_t ggo_moe_router_scratch_bytes(int64_t num_tokens, int num_experts);
+int ggo_moe_router(const void* logits_dev, int dtype, int64_t num_tokens, int num_experts,
+                   int top_k, const uint8_t* token_mask_dev, int32_t* topk_ids_dev,
+                   float* topk_weights_dev, int64_t* tokens_per_expert_dev,
+                   int64_t* balance_counts_dev, float* balance_loss_dev, float* row_stat_dev,
+                   float* coef_dev, void* scratch_dev, cudaStream_t stream);
+
+/* Gradient of ggo_moe_router: grad_logits_dev [T, E] (logits' dtype) from grad_weights_dev [T, top_k]
+ * fp32 and grad_loss_dev (one fp32 in device memory), either of which may be NULL (zero); the other
+ * inputs as ggo_moe_router read or wrote them. Written, not added to. */
+int ggo_moe_router_backward(const void* logits_dev, int dtype, int64_t num_tokens, int num_experts,
+                            int top_k, const int32_t* topk_ids_dev, const float* topk_weights_dev,
+                            const float* row_stat_dev, const float* coef_dev,
+                            const float* grad_weights_dev, const float* grad_loss_dev,
+                            void* grad_logits_dev, cudaStream_t stream);
+
+/* Fused-MoE stage 1b for INT8 experts: ggo_moe_permute with ggo_quantize_int8_rows on the way. Each
+ * token's row is coded once and its codes are written to the token's top_k sorted rows
+ * q_sorted_dev [T*top_k, H], its scale to scale_sorted_dev [T*top_k]; slot_pos_dev as there.
+ * scratch_dev from ggo_moe_route or ggo_moe_router on the same stream. H a multiple of 16. */
+int ggo_moe_permute_int8(const void* x_dev, int64_t num_tokens, int64_t hidden, int num_experts,
+                         int top_k, const int32_t* topk_ids_dev, void* q_sorted_dev,
+                         float* scale_sorted_dev, int32_t* slot_pos_dev, const void* scratch_dev,
+                         int dtype, cudaStream_t stream);
 
 /* Fused-MoE stage 1b: permute. Sorted order is expert-major, then token index (each token's k
  * experts are distinct, so the k-slot never ties). Writes
