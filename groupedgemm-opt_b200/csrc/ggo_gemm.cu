@@ -149,7 +149,9 @@ int launch(const void* a, const void* b, int64_t b_rows, const GemmParams& p, in
   if (OP != kOp16) {
     if (int st = make_map_byte(&ma, a, q.rows, q.k, kBM)) return st;
     if (int st = make_map_byte(&mb, b, b_rows, q.k, 128)) return st;
-    q.skinny_max = 0;
+    if (OP == kOpE4M3) q.skinny_max = 0;
+    if (q.skinny_max > 0)
+      if (int st = make_map_byte(&mas, a, q.rows, q.k, kSkinnyRows)) return st;
   } else {
     if (int st = make_map(&ma, a, q.rows, q.k, BF16, kBM)) return st;
     if (int st = make_b_map<BMN>(&mb, b, b_rows, q, BF16, 128)) return st;
@@ -327,8 +329,9 @@ int64_t mx_scale_atoms(int64_t rows, int64_t segments, int64_t k) {
   return ((rows + 127) / 128 + segments) * (k / 128);
 }
 
-// One-byte operands with the scaled epilogue: CTA-pair pass (+ short-tail pass) or single-CTA
-// 128x256 tiles.
+// One-byte operands with the scaled epilogue: CTA-pair pass (+ short-tail pass), or single-CTA
+// 128x256 tiles; the plain int8 product also 128x128 ones, where choose_bn finds that wide tiles
+// leave SMs idle.
 template <int EPI, bool BF16, int OP>
 int launch_scaled(const void* input, const void* weights, int64_t b_rows, GemmParams p, int bn,
                   int dev, cudaStream_t stream) {
@@ -344,6 +347,8 @@ int launch_scaled(const void* input, const void* weights, int64_t b_rows, GemmPa
     if (st || !split) return st;
     p.split_mode = 2;
   }
+  if constexpr (OP == kOpI8 && !epi_glu(EPI))
+    if (bn == 128) return launch<128, EPI, BF16, false, OP>(input, weights, b_rows, p, dev, stream);
   return launch<256, EPI, BF16, false, OP>(input, weights, b_rows, p, dev, stream);
 }
 

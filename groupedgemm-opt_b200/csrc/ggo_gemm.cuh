@@ -105,7 +105,7 @@ struct GemmParams {
   // Skinny tiles: a tile of at most this many rows (a short segment, or a segment's last rows)
   // runs with the operands swapped -- weight rows on the MMA's M side, the tile's rows on its N
   // side rounded up to 16 -- so the tensor cores do work for the rows that exist instead of a
-  // 128-row block. 0 disables. Single-CTA kernel, bf16/fp16 K-major weights, plain or SwiGLU.
+  // 128-row block. 0 disables. Single-CTA kernel, bf16/fp16 or int8 K-major weights.
   int skinny_max;
   GgoWorkspace* ws;
   int* err;  // where device errors are recorded (first one wins): &ws->error unless given apart
@@ -373,8 +373,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
   return *reinterpret_cast<uint32_t*>(&t2);
 }
 
-// 32 output columns of this thread's accumulator row, packed as 16 bf16x2/half2 words: TMEM
-// columns [c, c+32) (plain), or silu(gate) * up from columns [c, c+32) and [BN/2 + c, ...).
 // An accumulator word as fp32: already fp32, or (I8) a 32-bit integer sum, rounded to nearest (exact
 // up to 2^24).
 template <bool I8>
@@ -382,6 +380,26 @@ __device__ __forceinline__ float acc_to_float(uint32_t v) {
   return I8 ? __int2float_rn(static_cast<int>(v)) : __uint_as_float(v);
 }
 
+// silu(gate) * up of two accumulator words under their scales. The integer path divides by
+// multiplying with the hardware reciprocal (within 2 ulp, far below the rounding to 16 bits that
+// follows).
+template <bool I8>
+__device__ __forceinline__ float scaled_silu_mul(uint32_t g, uint32_t u, float rs, float cg,
+                                                 float cu) {
+  const float gv = acc_to_float<I8>(g) * rs * cg;
+  const float uv = acc_to_float<I8>(u) * rs * cu;
+  const float d = 1.0f + __expf(-gv);
+  return (I8 ? __fdividef(gv, d) : gv / d) * uv;
+}
+
+// Whether 32 column scales can be read as eight 16-byte words (warp-uniform): all of them exist and
+// the first is aligned.
+__device__ __forceinline__ bool scales_in_fours(const float* cs, int cs_valid) {
+  return cs_valid >= 32 && (reinterpret_cast<uintptr_t>(cs) & 15u) == 0;
+}
+
+// 32 output columns of this thread's accumulator row, packed as 16 bf16x2/half2 words: TMEM
+// columns [c, c+32) (plain), or silu(gate) * up from columns [c, c+32) and [BN/2 + c, ...).
 template <int BN, int EPI, bool BF16, bool I8 = false>
 __device__ __forceinline__ void load_out32(uint32_t t_row, int c, uint32_t (&o)[16], float rs = 1.f,
                                            const float* cs = nullptr, int cs_valid = 0,
@@ -391,6 +409,18 @@ __device__ __forceinline__ void load_out32(uint32_t t_row, int c, uint32_t (&o)[
     tmem_ld_32x32b_x32(t_row + c, g);
     tmem_ld_32x32b_x32(t_row + BN / 2 + c, u);
     tmem_ld_wait();
+    if (scales_in_fours(cs, cs_valid) && scales_in_fours(cs + cs_up_off, cs_valid)) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(cs) + q);
+        const float4 b = __ldg(reinterpret_cast<const float4*>(cs + cs_up_off) + q);
+        o[2 * q] = pack2(scaled_silu_mul<I8>(g[4 * q], u[4 * q], rs, a.x, b.x),
+                         scaled_silu_mul<I8>(g[4 * q + 1], u[4 * q + 1], rs, a.y, b.y), BF16);
+        o[2 * q + 1] = pack2(scaled_silu_mul<I8>(g[4 * q + 2], u[4 * q + 2], rs, a.z, b.z),
+                             scaled_silu_mul<I8>(g[4 * q + 3], u[4 * q + 3], rs, a.w, b.w), BF16);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float y[2];
@@ -398,9 +428,8 @@ __device__ __forceinline__ void load_out32(uint32_t t_row, int c, uint32_t (&o)[
       for (int e = 0; e < 2; ++e) {
         const int j = 2 * i + e;
         const bool ok = j < cs_valid;
-        const float gv = acc_to_float<I8>(g[j]) * rs * (ok ? __ldg(cs + j) : 0.f);
-        const float uv = acc_to_float<I8>(u[j]) * rs * (ok ? __ldg(cs + cs_up_off + j) : 0.f);
-        y[e] = gv / (1.0f + __expf(-gv)) * uv;
+        y[e] = scaled_silu_mul<I8>(g[j], u[j], rs, ok ? __ldg(cs + j) : 0.f,
+                                   ok ? __ldg(cs + cs_up_off + j) : 0.f);
       }
       o[i] = pack2(y[0], y[1], BF16);
     }
@@ -408,6 +437,17 @@ __device__ __forceinline__ void load_out32(uint32_t t_row, int c, uint32_t (&o)[
     uint32_t v[32];
     tmem_ld_32x32b_x32(t_row + c, v);
     tmem_ld_wait();
+    if (scales_in_fours(cs, cs_valid)) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(cs) + q);
+        o[2 * q] = pack2(acc_to_float<I8>(v[4 * q]) * rs * a.x,
+                         acc_to_float<I8>(v[4 * q + 1]) * rs * a.y, BF16);
+        o[2 * q + 1] = pack2(acc_to_float<I8>(v[4 * q + 2]) * rs * a.z,
+                             acc_to_float<I8>(v[4 * q + 3]) * rs * a.w, BF16);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const float s0 = 2 * i < cs_valid ? __ldg(cs + 2 * i) : 0.f;
@@ -595,19 +635,30 @@ __device__ __forceinline__ OutT* output_row(const GemmParams& p, const TileInfo&
 // row, column = the tile's input row. The warp holding lanes [32 ew, 32 ew + 32) of weight half h
 // (TMEM columns [128 h, 128 h + 64)) owns output columns n0 + 128 h + 32 ew + lane (plain), or
 // n0 + 32 ew + lane with gate in half 0 and up in half 1 (SwiGLU). For every input row of the
-// tile the 32 lanes store 32 consecutive output columns (64 contiguous bytes). All 32 lanes must
-// call it (tcgen05.ld is warp-collective).
-template <int BN, int EPI, bool BF16, typename OutT>
+// tile the 32 lanes store 32 consecutive output columns (64 contiguous bytes). Scaled epilogues: a
+// lane's column scales stay with it, lane j of the warp reads the scale of input row j. All 32 lanes
+// must call it (tcgen05.ld is warp-collective).
+template <int BN, int EPI, bool BF16, typename OutT, bool I8>
 __device__ __forceinline__ void store_skinny(uint32_t t_row, const GemmParams& p,
                                              const TileInfo& info, int ew) {
+  constexpr bool kScaled = EPI == kEpiScaled || EPI == kEpiScaledSwiGLU;
   const int lane = threadIdx.x & 31;
   constexpr int kHalves = epi_glu(EPI) ? 1 : BN / 128;
 #pragma unroll 1
   for (int h = 0; h < kHalves; ++h) {
     const int col = info.n0 + 128 * h + 32 * ew + lane;
     const bool col_ok = col < p.n_out;
+    float cs = 0.f, cu = 0.f;
+    if (kScaled && col_ok) {
+      const float* scales = p.col_scale + static_cast<size_t>(info.seg % p.num_experts) * p.n_b;
+      cs = __ldg(scales + col);
+      if (epi_glu(EPI)) cu = __ldg(scales + p.n_b / 2 + col);
+    }
 #pragma unroll 1
     for (int cb = 0; cb < info.rows; cb += 32) {
+      float row_scale = 0.f;
+      if (kScaled && cb + lane < info.rows && info.row0 + cb + lane < p.rows)
+        row_scale = __ldg(p.row_scale + info.row0 + cb + lane);
       uint32_t v[32];
       uint32_t u[32];
       tmem_ld_32x32b_x32(t_row + 128 * h + cb, v);
@@ -617,8 +668,15 @@ __device__ __forceinline__ void store_skinny(uint32_t t_row, const GemmParams& p
       for (int j = 0; j < 32; ++j) {
         const int r = cb + j;
         const bool ok = r < info.rows && info.row0 + r < p.rows;
-        float y = __uint_as_float(v[j]);
-        if (epi_glu(EPI)) y = y / (1.0f + __expf(-y)) * __uint_as_float(u[j]);
+        float y;
+        if (kScaled) {
+          const float rs = __shfl_sync(0xffffffffu, row_scale, j);
+          y = epi_glu(EPI) ? scaled_silu_mul<I8>(v[j], u[j], rs, cs, cu)
+                           : acc_to_float<I8>(v[j]) * rs * cs;
+        } else {
+          y = __uint_as_float(v[j]);
+          if (epi_glu(EPI)) y = y / (1.0f + __expf(-y)) * __uint_as_float(u[j]);
+        }
         OutT* dst = output_row<OutT>(p, info, r, ok);
         if (ok && col_ok) dst[col] = static_cast<OutT>(y);
       }
@@ -638,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kOutBN = epi_glu(EPI) ? BN / 2 : BN;
   constexpr bool kTmaStoreOk = kOutBN % 64 == 0;  // output boxes are 64 columns wide
   // skinny tiles: tmAs is the input map with kSkinnyRows-row boxes
-  constexpr bool kSkinnyOk = OP == kOp16 && !BMN && (EPI == kEpiStore || EPI == kEpiSwiGLU);
+  constexpr bool kSkinnyOk = !BMN && OP != kOpE4M3;
   constexpr int kSkinnyABytes = kSkinnyRows * kBK * 2;
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -771,7 +829,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool valid = ring[q].rows > 0;
         const bool skinny = kSkinnyOk && ring[q].skinny;
         // skinny: M = 128 weight rows per MMA, N = the tile's rows rounded up to 16
-        const uint32_t idesc_s = idesc_f16(kBM, (ring[q].rows + 15) & ~15, BF16, false);
+        const int n_s = (ring[q].rows + 15) & ~15;
+        const uint32_t idesc_s = OP == kOpI8 ? idesc_i8(kBM, n_s)
+                                             : idesc_f16(kBM, n_s, BF16, false);
         mbar_arrive(&sche_bar[q]);
         if (++q == kSchedDepth) { q = 0; qphase ^= 1; }
         if (!valid) break;
@@ -798,10 +858,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
 #pragma unroll
-              for (int h = 0; h < BN / 128; ++h)
-                mma_f16_ss(d_tmem + 128 * h,
-                           sdesc_sw128_kmajor(a_addr + L::kABytes + h * 16384) + 2 * kk,
-                           adesc + 2 * kk, idesc_s, (kb | kk) != 0);
+              for (int h = 0; h < BN / 128; ++h) {
+                const uint64_t wdesc =
+                    sdesc_sw128_kmajor(a_addr + L::kABytes + h * 16384) + 2 * kk;
+                if (OP == kOpI8)
+                  mma_i8_ss(d_tmem + 128 * h, wdesc, adesc + 2 * kk, idesc_s, (kb | kk) != 0);
+                else
+                  mma_f16_ss(d_tmem + 128 * h, wdesc, adesc + 2 * kk, idesc_s, (kb | kk) != 0);
+              }
             }
             mma_commit(&empty_bar[stage]);
             if (++stage == S) { stage = 0; phase ^= 1; }
@@ -842,7 +906,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + acc * BN;
       using OutT = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
       if (kSkinnyOk && info.skinny) {
-        store_skinny<BN, EPI, BF16, OutT>(t_row, p, info, ew);
+        store_skinny<BN, EPI, BF16, OutT, OP == kOpI8>(t_row, p, info, ew);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&acce_bar[acc]);
