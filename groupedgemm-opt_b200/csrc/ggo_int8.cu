@@ -165,24 +165,29 @@ __global__ void __launch_bounds__(256)
 }
 
 // The dispatch's permutation with the quantisation on the way: every token's row is read, coded
-// once and written to its top_k expert-sorted places as codes. grid = (ceil(T / 32), kSplit): block
+// once and written to its top_k expert-sorted places as codes. grid = (ceil(T / 32), 4 WPT): block
 // (b, s) finds the sorted positions of 32-token block b (one warp walks its (token, slot) entries
-// in order, as the bf16 dispatch does) and moves the tokens congruent to s mod kSplit, one warp each.
-constexpr int kSplit = 4;
-
-template <typename T16>
+// in order, as the bf16 dispatch does) and moves the tokens congruent to s mod 4 WPT, WPT warps each:
+// one, or all eight when there are too few tokens to give every SM eight rows.
+template <typename T16, int WPT>
 __global__ void __launch_bounds__(256)
     permute_int8_kernel(const T16* __restrict__ x, int T, int H, int E, int K,
                         const int32_t* __restrict__ topk_ids, const int* __restrict__ block_offsets,
                         uint8_t* __restrict__ q_sorted, float* __restrict__ scale_sorted,
                         int32_t* __restrict__ slot_pos) {
   extern __shared__ int psm[];
+  __shared__ uint32_t s_max[8];
   int* off = psm;      // [E] running sorted position per expert
   int* pos = psm + E;  // [kRouteTokens * K]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t0 = blockIdx.x * kRouteTokens;
   const int ntok = min(kRouteTokens, T - t0);
   const int nent = ntok * K;
+  const int vec = H / 8;
+  constexpr int kStep = 32 * WPT;  // columns (of 16 bytes) between a thread's pieces of a row
+  const int col = WPT == 1 ? lane : static_cast<int>(threadIdx.x);
+  const int tl = (WPT == 1 ? warp * 4 : 0) + blockIdx.y;
+  const uint4* src = reinterpret_cast<const uint4*>(x + static_cast<size_t>(t0 + tl) * H);
   for (int e = threadIdx.x; e < E; e += 256)
     off[e] = block_offsets[static_cast<size_t>(blockIdx.x) * E + e];
   __syncthreads();
@@ -205,21 +210,26 @@ __global__ void __launch_bounds__(256)
       __syncwarp();
     }
   }
-  __syncthreads();
-  const int vec = H / 8;
-  for (int tl = warp * kSplit + blockIdx.y; tl < ntok; tl += 8 * kSplit) {
-    const uint4* src = reinterpret_cast<const uint4*>(x + static_cast<size_t>(t0 + tl) * H);
-    uint32_t m = 0;
+  uint32_t m = 0;
+  if (tl < ntok) {
 #pragma unroll 8
-    for (int c = lane; c < vec; c += 32) m = abs_max8(m, src[c]);
-    const RowCode rc = row_code<T16>(warp_max2(m));
-    for (int j = lane; j < K; j += 32) scale_sorted[pos[tl * K + j]] = rc.scale;
+    for (int c = col; c < vec; c += kStep) m = abs_max8(m, src[c]);
+  }
+  m = warp_max2(m);
+  if (WPT > 1 && lane == 0) s_max[warp] = m;
+  __syncthreads();
+  if (tl >= ntok) return;
+  if (WPT > 1) {
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = __vmaxu2(m, s_max[w]);
+  }
+  const RowCode rc = row_code<T16>(m);
+  if (col < K) scale_sorted[pos[tl * K + col]] = rc.scale;
 #pragma unroll 4
-    for (int c = lane; c < vec; c += 32) {
-      const uint2 o = code8<T16>(src[c], rc);
-      for (int j = 0; j < K; ++j)
-        reinterpret_cast<uint2*>(q_sorted + static_cast<size_t>(pos[tl * K + j]) * H)[c] = o;
-    }
+  for (int c = col; c < vec; c += kStep) {
+    const uint2 o = code8<T16>(src[c], rc);
+    for (int j = 0; j < K; ++j)
+      reinterpret_cast<uint2*>(q_sorted + static_cast<size_t>(pos[tl * K + j]) * H)[c] = o;
   }
 }
 
@@ -242,10 +252,15 @@ template <typename T16>
 int launch_permute(const void* x, int T, int H, int E, int K, const int32_t* ids,
                    const int* offsets, uint8_t* q, float* scale, int32_t* slot_pos,
                    cudaStream_t stream) {
-  const dim3 grid((T + kRouteTokens - 1) / kRouteTokens, kSplit);
+  const int nb = (T + kRouteTokens - 1) / kRouteTokens;
   const size_t smem = (static_cast<size_t>(E) + kRouteTokens * K) * 4;  // at most 6 KB
-  permute_int8_kernel<T16><<<grid, 256, smem, stream>>>(static_cast<const T16*>(x), T, H, E, K, ids,
-                                                        offsets, q, scale, slot_pos);
+  const T16* xp = static_cast<const T16*>(x);
+  if (4 * nb <= 148)
+    permute_int8_kernel<T16, 8><<<dim3(nb, 32), 256, smem, stream>>>(xp, T, H, E, K, ids, offsets, q,
+                                                                   scale, slot_pos);
+  else
+    permute_int8_kernel<T16, 1><<<dim3(nb, 4), 256, smem, stream>>>(xp, T, H, E, K, ids, offsets, q,
+                                                                  scale, slot_pos);
   return check_launch();
 }
 

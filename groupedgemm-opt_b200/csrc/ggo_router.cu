@@ -23,22 +23,46 @@ namespace ggo {
 namespace {
 
 constexpr int kTokens = 32;    // tokens per block: the granularity of the dispatch's offset table
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 constexpr int kMaxE = 1024;
 constexpr int kMaxK = 16;
 constexpr unsigned kAll = 0xffffffffu;
 
 // Monotone float -> uint32 (larger float -> larger key). -0 counts as +0 and NaN as the largest, so
-// that equal floats have equal keys; 0 is below every key and marks a chosen or absent expert.
+// that equal floats have equal keys; no float has key 0.
 __device__ __forceinline__ uint32_t order_key(float f) {
   if (f != f) return 0xffffffffu;
   const uint32_t b = __float_as_uint(f + 0.0f);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-__device__ __forceinline__ float key_value(uint32_t k) {
-  if (k == 0xffffffffu) return __int_as_float(0x7fc00000);
-  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+
+// A logit's key and its expert in one word, larger for larger logits and, among equal keys, for
+// lower experts, so that a plain maximum chooses. The 16-bit types' keys are whole (upper half);
+// fp32 keys lose their low 8 or 10 bits to the expert (IDX bits), which choose_top_k makes good.
+template <typename TL>
+struct KeyBits {
+  static constexpr bool kWhole = true;
+};
+template <>
+struct KeyBits<float> {
+  static constexpr bool kWhole = false;
+};
+
+template <typename TL, int V>
+__device__ __forceinline__ uint32_t packed_key(TL x, int e) {
+  const float f = static_cast<float>(x);
+  if constexpr (KeyBits<TL>::kWhole) {
+    uint32_t b = *reinterpret_cast<const unsigned short*>(&x);
+    if ((b & 0x7fffu) == 0) b = 0;  // -0 as +0
+    const uint32_t key = f != f ? 0xffffu : ((b & 0x8000u) ? (~b & 0xffffu) : (b | 0x8000u));
+    return (key << 16) | (0xffffu - static_cast<uint32_t>(e));
+  } else {
+    constexpr uint32_t kIdx = V <= 8 ? 0xffu : 0x3ffu;
+    return (order_key(f) & ~kIdx) | (kIdx - static_cast<uint32_t>(e));
+  }
+}
+template <typename TL, int V>
+__device__ __forceinline__ uint32_t index_mask() {
+  return KeyBits<TL>::kWhole ? 0xffffu : (V <= 8 ? 0xffu : 0x3ffu);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -47,61 +71,151 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
-                   : "memory");
+// Expert of a lane's i-th value: neighbouring experts on neighbouring lanes, or (VEC, E == 32 V) V
+// neighbouring experts per lane, which are then loaded and stored 16 bytes at a time.
+template <int V, bool VEC>
+__device__ __forceinline__ int expert_of(int lane, int i) {
+  return VEC ? lane * V + i : lane + 32 * i;
 }
 
-// One warp per token, lane l holding experts l, l + 32, ... (V of them). grid = ceil(T / kTokens).
-// table[b][e] receives block b's choices of expert e, all in the low and kept in the high 16 bits;
-// psum[b][e] the block's sum of P over kept tokens; row_stat[t] = (max logit, 1 / sum exp(l - max)),
-// the second 0 for tokens that are not kept.
+// A lane's values of one row of logits; values behind E are not defined.
+template <typename TL, int V, bool VEC>
+__device__ __forceinline__ void load_row(const TL* __restrict__ row, int E, int lane, TL (&x)[V]) {
+  if constexpr (VEC) {
+    constexpr int kBytes = V * static_cast<int>(sizeof(TL));
+    const char* src = reinterpret_cast<const char*>(row) + lane * kBytes;
+    if constexpr (kBytes >= 16) {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i)
+        reinterpret_cast<uint4*>(x)[i] = reinterpret_cast<const uint4*>(src)[i];
+    } else if constexpr (kBytes == 8) {
+      *reinterpret_cast<uint2*>(x) = *reinterpret_cast<const uint2*>(src);
+    } else {
+      *reinterpret_cast<uint32_t*>(x) = *reinterpret_cast<const uint32_t*>(src);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (lane + 32 * i < E) x[i] = row[lane + 32 * i];
+  }
+}
+
+// The K largest logits of a row, lane j getting expert and logit of the j-th, by K maxima over the
+// warp of whole (key, expert) pairs: exact for every input, and slow.
 template <typename TL, int V>
-__global__ void __launch_bounds__(kThreads)
+__device__ __noinline__ int choose_exactly(const TL* __restrict__ row, int E, int K, int lane) {
+  uint32_t key[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    key[i] = lane + 32 * i < E ? order_key(static_cast<float>(row[lane + 32 * i])) : 0u;
+  int id = 0;
+  for (int j = 0; j < K; ++j) {
+    uint32_t m = key[0];
+#pragma unroll
+    for (int i = 1; i < V; ++i) m = max(m, key[i]);
+    const uint32_t best = __reduce_max_sync(kAll, m);
+    int e_min = kMaxE;
+#pragma unroll
+    for (int i = V - 1; i >= 0; --i)
+      if (key[i] == best) e_min = lane + 32 * i;
+    const int chosen = __reduce_min_sync(kAll, e_min);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (lane + 32 * i == chosen) key[i] = 0u;
+    if (lane == j) id = chosen;
+  }
+  return id;
+}
+
+// Sorts a lane's V words in descending order (Batcher's odd-even merge sort; V a power of two).
+template <int V>
+__device__ __forceinline__ void sort_descending(uint32_t (&k)[V]) {
+#pragma unroll
+  for (int p = 1; p < V; p *= 2)
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+      for (int j = q % p; j + q < V; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < V && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const uint32_t hi = max(k[i + j], k[i + j + q]), lo = min(k[i + j], k[i + j + q]);
+            k[i + j] = hi;
+            k[i + j + q] = lo;
+          }
+}
+
+// The expert (lane j: the j-th choice) of the K largest of the warp's packed keys. With V <= 8 every
+// lane sorts its keys once and the warp takes K times the largest head; longer lists are searched
+// each time. fp32: a lost key bit matters only where two neighbours of the order, up to the first
+// one not chosen, share the kept bits; then the row is chosen again with whole keys.
+template <typename TL, int V>
+__device__ __forceinline__ int choose_top_k(uint32_t (&k)[V], const TL* __restrict__ row, int E,
+                                            int K, int lane) {
+  constexpr bool kSorted = V <= 8;
+  const uint32_t idx = index_mask<TL, V>();
+  if constexpr (kSorted) sort_descending<V>(k);
+  uint32_t mine = 0;
+  const int rounds = KeyBits<TL>::kWhole ? K : K + 1;
+  for (int j = 0; j < rounds; ++j) {
+    uint32_t m = k[0];
+    if constexpr (!kSorted) {
+#pragma unroll
+      for (int i = 1; i < V; ++i) m = max(m, k[i]);
+    }
+    const uint32_t best = __reduce_max_sync(kAll, m);
+    if constexpr (kSorted) {
+      const bool pop = m == best;
+#pragma unroll
+      for (int i = 0; i + 1 < V; ++i) k[i] = pop ? k[i + 1] : k[i];
+      k[V - 1] = pop ? 0u : k[V - 1];
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) k[i] = k[i] == best ? 0u : k[i];
+    }
+    if (lane == j) mine = best;
+  }
+  int id = static_cast<int>(idx - (mine & idx));
+  if constexpr (!KeyBits<TL>::kWhole) {
+    const uint32_t next = __shfl_down_sync(kAll, mine, 1);
+    const bool unsure = lane < K && ((mine ^ next) & ~idx) == 0;
+    if (__any_sync(kAll, unsure)) id = choose_exactly<TL, V>(row, E, K, lane);
+  }
+  return id;
+}
+
+// One warp per token. grid = ceil(T / kTokens), NW warps: 8, or 32 (a token each) when the blocks
+// would not fill the GPU. table[b][e] receives block b's choices of expert e, all in the low and
+// kept in the high 16 bits; psum[b][e] the block's sum of P over kept tokens; row_stat[t] =
+// (max logit, 1 / sum exp(l - max)), the second 0 for tokens that are not kept.
+template <typename TL, int V, bool VEC, int NW>
+__global__ void __launch_bounds__(32 * NW)
     router_kernel(const TL* __restrict__ logits, const uint8_t* __restrict__ mask, int T, int E,
                   int K, int32_t* __restrict__ ids, float* __restrict__ weights,
                   float2* __restrict__ row_stat, uint32_t* __restrict__ table,
                   float* __restrict__ psum) {
   extern __shared__ uint32_t sm[];
   uint32_t* hist = sm;                                    // [E]
-  float* wsum = reinterpret_cast<float*>(sm + E);         // [kWarps][E]
+  float* wsum = reinterpret_cast<float*>(sm + E);         // [NW][E]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int e = threadIdx.x; e < E; e += kThreads) hist[e] = 0;
+  for (int e = threadIdx.x; e < E; e += 32 * NW) hist[e] = 0;
   __syncthreads();
   float acc[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
   const int t0 = blockIdx.x * kTokens;
-  for (int t = t0 + warp; t < min(T, t0 + kTokens); t += kWarps) {
+  for (int t = t0 + warp; t < min(T, t0 + kTokens); t += NW) {
     const TL* row = logits + static_cast<size_t>(t) * E;
-    float l[V];
+    alignas(16) TL x[V];
+    load_row<TL, V, VEC>(row, E, lane, x);
     uint32_t key[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int e = lane + 32 * i;
-      l[i] = e < E ? static_cast<float>(row[e]) : -INFINITY;
-      key[i] = e < E ? order_key(l[i]) : 0u;
+      const int e = expert_of<V, VEC>(lane, i);
+      key[i] = (VEC || e < E) ? packed_key<TL, V>(x[i], e) : 0u;
     }
-    float val = 0.f;  // lane j: the j-th choice
-    int id = 0;
-    for (int j = 0; j < K; ++j) {
-      uint32_t m = key[0];
-#pragma unroll
-      for (int i = 1; i < V; ++i) m = max(m, key[i]);
-      const uint32_t best = __reduce_max_sync(kAll, m);
-      int e_min = kMaxE;
-#pragma unroll
-      for (int i = V - 1; i >= 0; --i)
-        if (key[i] == best) e_min = lane + 32 * i;
-      const int chosen = __reduce_min_sync(kAll, e_min);
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (lane + 32 * i == chosen) key[i] = 0u;
-      if (lane == j) {
-        val = key_value(best);
-        id = chosen;
-      }
-    }
+    const int id = choose_top_k<TL, V>(key, row, E, K, lane);
+    const float val = lane < K ? static_cast<float>(row[id]) : 0.f;
     const float top = __shfl_sync(kAll, val, 0);
     const bool live = top != -INFINITY;
     const bool kept = live && (mask == nullptr || mask[t] != 0);
@@ -118,29 +232,37 @@ __global__ void __launch_bounds__(kThreads)
     // softmax over all experts
     float inv = 0.f;
     if (kept) {
+      float p[V];
       float z = 0.f;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        l[i] = expf(l[i] - top);
-        z += l[i];
+        p[i] = (VEC || lane + 32 * i < E) ? expf(static_cast<float>(x[i]) - top) : 0.f;
+        z += p[i];
       }
       inv = 1.0f / warp_sum(z);
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] = fmaf(l[i], inv, acc[i]);
+      for (int i = 0; i < V; ++i) acc[i] = fmaf(p[i], inv, acc[i]);
     }
     if (lane == 0) row_stat[t] = make_float2(live ? top : 0.f, inv);
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-    if (lane + 32 * i < E) wsum[warp * E + lane + 32 * i] = acc[i];
+  for (int i = 0; i < V; ++i) {
+    const int e = expert_of<V, VEC>(lane, i);
+    if (VEC || e < E) wsum[warp * E + e] = acc[i];
+  }
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += kThreads) {
+  for (int e = threadIdx.x; e < E; e += 32 * NW) {
     float p = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) p += wsum[w * E + e];
+    for (int w = 0; w < NW; ++w) p += wsum[w * E + e];
     psum[static_cast<size_t>(blockIdx.x) * E + e] = p;
     table[static_cast<size_t>(blockIdx.x) * E + e] = hist[e];
   }
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
 }
 
 // One cluster of up to 8 CTAs x 1024 threads; CTA r owns experts [r * CE, (r+1) * CE). Thread
@@ -160,7 +282,8 @@ __global__ void __launch_bounds__(1024)
   __shared__ int tot_kept[kMaxE];
   __shared__ double tot_p[kMaxE];
   __shared__ int start[kMaxE];
-  __shared__ double red[1024];
+  __shared__ int warp_tot[32], warp_kept[32];
+  __shared__ double warp_term[32];
   unsigned rank, ncta;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ncta));
@@ -212,21 +335,41 @@ __global__ void __launch_bounds__(1024)
     }
   }
   cluster_barrier();
-  // exclusive scan of the totals over experts, and the sum of kept choices (every CTA alike)
-  start[tid] = tid < E ? tot[tid] : 0;
-  part_kept[tid] = tid < E ? tot_kept[tid] : 0;
-  __syncthreads();
-  for (int o = 1; o < E; o <<= 1) {
-    const int v = tid >= o ? start[tid - o] : 0;
-    const int k = tid >= o ? part_kept[tid - o] : 0;
-    __syncthreads();
-    start[tid] += v;
-    part_kept[tid] += k;
-    __syncthreads();
+  // exclusive scan of the totals over experts, the sum of kept choices and the loss (every CTA
+  // alike): within warps, then over the warps' sums
+  const int lane = tid & 31, wid = tid >> 5;
+  const int mine = tid < E ? tot[tid] : 0;
+  const int mine_kept = tid < E ? tot_kept[tid] : 0;
+  double term = tid < E ? static_cast<double>(mine_kept) * tot_p[tid] : 0.0;
+  int scan = mine, ksum = mine_kept;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(kAll, scan, o);
+    if (lane >= o) scan += v;
   }
-  const long long choices = part_kept[E - 1];  // top_k T'
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    ksum += __shfl_xor_sync(kAll, ksum, o);
+    term += __shfl_xor_sync(kAll, term, o);
+  }
+  if (lane == 31) {
+    warp_tot[wid] = scan;
+    warp_kept[wid] = ksum;
+    warp_term[wid] = term;
+  }
+  __syncthreads();
+  int before = 0;
+  long long choices = 0;  // top_k T'
+  double sum_np = 0.0;    // sum_e n_e sum_t P
+  for (int w = 0; w < (E + 31) / 32; ++w) {
+    if (w < wid) before += warp_tot[w];
+    choices += warp_kept[w];
+    sum_np += warp_term[w];
+  }
+  start[tid] = before + scan - mine;
+  __syncthreads();
   if (active) {
-    const int first = start[e] - tot[e];
+    const int first = start[e];
     if (q == 0) reinterpret_cast<int*>(table)[static_cast<size_t>(nblocks) * E + e] = first;
     int run = first + part_all[tid];
 #pragma unroll 8
@@ -238,30 +381,24 @@ __global__ void __launch_bounds__(1024)
     }
   }
   if (rank == 0) {
-    const double kept_tokens = static_cast<double>(choices) / K;
-    double term = 0.0;
+    // loss = E sum_e (n_e / choices) (sum_t P / T'), coef_e = E (n_e / choices) / T'
+    const double scale =
+        choices > 0 ? static_cast<double>(E) * K / (static_cast<double>(choices) * choices) : 0.0;
     if (tid < E) {
-      tpe[tid] = tot[tid];
-      kept_counts[tid] = tot_kept[tid];
-      const double f = choices > 0 ? static_cast<double>(tot_kept[tid]) / choices : 0.0;
-      term = choices > 0 ? E * f * tot_p[tid] / kept_tokens : 0.0;
-      coef[tid] = choices > 0 ? static_cast<float>(E * f / kept_tokens) : 0.f;
+      tpe[tid] = mine;
+      kept_counts[tid] = mine_kept;
+      coef[tid] = static_cast<float>(scale * mine_kept);
     }
-    red[tid] = term;
-    __syncthreads();
-    for (int o = 512; o > 0; o >>= 1) {
-      if (o >= E) continue;  // nothing but zeros behind E
-      if (tid < o) red[tid] += red[tid + o];
-      __syncthreads();
-    }
-    if (tid == 0) *loss = static_cast<float>(red[0]);
+    if (tid == 0) *loss = static_cast<float>(scale * sum_np);
   }
 }
 
 // One warp per token, persistent over tokens so that a lane's coefficients stay in registers. Every
 // warp owns E floats of shared memory in which the k choices' gradients are laid out by expert.
-template <typename TL, int V>
-__global__ void __launch_bounds__(kThreads)
+constexpr int kBwdWarps = 8;
+
+template <typename TL, int V, bool VEC>
+__global__ void __launch_bounds__(32 * kBwdWarps)
     router_backward_kernel(const TL* __restrict__ logits, const float2* __restrict__ row_stat,
                            const int32_t* __restrict__ ids, const float* __restrict__ weights,
                            const float* __restrict__ coef, const float* __restrict__ grad_w,
@@ -274,20 +411,15 @@ __global__ void __launch_bounds__(kThreads)
   const float gl = grad_loss ? *grad_loss : 0.f;
   float cf[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) cf[i] = lane + 32 * i < E ? gl * coef[lane + 32 * i] : 0.f;
+  for (int i = 0; i < V; ++i) {
+    const int e = expert_of<V, VEC>(lane, i);
+    cf[i] = (VEC || e < E) ? gl * coef[e] : 0.f;
+  }
   __syncwarp();
-  for (int t = blockIdx.x * kWarps + warp; t < T; t += gridDim.x * kWarps) {
-    const TL* row = logits + static_cast<size_t>(t) * E;
+  for (int t = blockIdx.x * kBwdWarps + warp; t < T; t += gridDim.x * kBwdWarps) {
     const float2 st = row_stat[t];
-    float p[V];
-    float dot = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = lane + 32 * i;
-      p[i] = (e < E && st.y != 0.f) ? expf(static_cast<float>(row[e]) - st.x) * st.y : 0.f;
-      dot = fmaf(p[i], cf[i], dot);
-    }
-    dot = warp_sum(dot);
+    alignas(16) TL x[V];
+    load_row<TL, V, VEC>(logits + static_cast<size_t>(t) * E, E, lane, x);
     int id = 0;
     if (grad_w) {
       float w = 0.f, u = 0.f;
@@ -300,11 +432,37 @@ __global__ void __launch_bounds__(kThreads)
       if (lane < K) add[id] = w * (u - mean);
       __syncwarp();
     }
+    float p[V];
+    float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int e = lane + 32 * i;
-      if (e < E)
-        out[static_cast<size_t>(t) * E + e] = static_cast<TL>(fmaf(p[i], cf[i] - dot, add[e]));
+      const bool some = (VEC || lane + 32 * i < E) && st.y != 0.f;
+      p[i] = some ? expf(static_cast<float>(x[i]) - st.x) * st.y : 0.f;
+      dot = fmaf(p[i], cf[i], dot);
+    }
+    dot = warp_sum(dot);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int e = expert_of<V, VEC>(lane, i);
+      if (VEC || e < E) x[i] = static_cast<TL>(fmaf(p[i], cf[i] - dot, add[e]));
+    }
+    TL* dst = out + static_cast<size_t>(t) * E;
+    if constexpr (VEC) {
+      constexpr int kBytes = V * static_cast<int>(sizeof(TL));
+      char* d = reinterpret_cast<char*>(dst) + lane * kBytes;
+      if constexpr (kBytes >= 16) {
+#pragma unroll
+        for (int i = 0; i < kBytes / 16; ++i)
+          reinterpret_cast<uint4*>(d)[i] = reinterpret_cast<const uint4*>(x)[i];
+      } else if constexpr (kBytes == 8) {
+        *reinterpret_cast<uint2*>(d) = *reinterpret_cast<const uint2*>(x);
+      } else {
+        *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const uint32_t*>(x);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (lane + 32 * i < E) dst[lane + 32 * i] = x[i];
     }
     if (grad_w) {
       __syncwarp();
@@ -316,12 +474,56 @@ __global__ void __launch_bounds__(kThreads)
 
 int blocks_for(int64_t T) { return static_cast<int>((T + kTokens - 1) / kTokens); }
 
+// Sixteen-byte access to rows needs rows and base on 16-byte boundaries: E == 32 V with at least four
+// bytes per lane, on an aligned tensor.
+template <typename TL, int V>
+bool vec_rows(const void* a, const void* b, int E) {
+  return E == 32 * V && V * sizeof(TL) >= 4 &&
+         ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15u) == 0;
+}
+
+template <typename TL, int V, bool VEC, int NW>
+int launch_router_as(const void* logits, const uint8_t* mask, int T, int E, int K, int32_t* ids,
+                     float* w, float2* stat, uint32_t* table, float* psum, cudaStream_t stream) {
+  const size_t smem = static_cast<size_t>(E) * (1 + NW) * 4;  // at most 36 KB
+  router_kernel<TL, V, VEC, NW><<<blocks_for(T), 32 * NW, smem, stream>>>(
+      static_cast<const TL*>(logits), mask, T, E, K, ids, w, stat, table, psum);
+  return check_launch();
+}
+
+// A warp per token while the blocks find free SMs; beyond that eight warps of four tokens each.
+// 256 tokens x 256 experts, fp32: 5.6 us against 16.5 us with eight warps of four tokens.
+constexpr int kWideBlocks = 148;
+
+template <typename TL, int V, bool VEC>
+int launch_router_vec(const void* logits, const uint8_t* mask, int T, int E, int K, int32_t* ids,
+                      float* w, float2* stat, uint32_t* table, float* psum, cudaStream_t stream) {
+  if constexpr (V <= 8)
+    if (blocks_for(T) <= kWideBlocks)
+      return launch_router_as<TL, V, VEC, 32>(logits, mask, T, E, K, ids, w, stat, table, psum,
+                                              stream);
+  return launch_router_as<TL, V, VEC, 8>(logits, mask, T, E, K, ids, w, stat, table, psum, stream);
+}
+
 template <typename TL, int V>
 int launch_router(const void* logits, const uint8_t* mask, int T, int E, int K, int32_t* ids,
                   float* w, float2* stat, uint32_t* table, float* psum, cudaStream_t stream) {
-  const size_t smem = static_cast<size_t>(E) * (1 + kWarps) * 4;  // at most 36 KB
-  router_kernel<TL, V><<<blocks_for(T), kThreads, smem, stream>>>(
-      static_cast<const TL*>(logits), mask, T, E, K, ids, w, stat, table, psum);
+  if constexpr (V * sizeof(TL) >= 4)
+    if (vec_rows<TL, V>(logits, nullptr, E))
+      return launch_router_vec<TL, V, true>(logits, mask, T, E, K, ids, w, stat, table, psum,
+                                            stream);
+  return launch_router_vec<TL, V, false>(logits, mask, T, E, K, ids, w, stat, table, psum, stream);
+}
+
+template <typename TL, int V, bool VEC>
+int launch_backward_as(const void* logits, const float2* stat, const int32_t* ids, const float* w,
+                       const float* coef, const float* gw, const float* gl, int T, int E, int K,
+                       void* out, cudaStream_t stream) {
+  const size_t smem = static_cast<size_t>(E) * kBwdWarps * 4;
+  const int want = (T + kBwdWarps - 1) / kBwdWarps;
+  const int grid = want < 148 * 8 ? want : 148 * 8;
+  router_backward_kernel<TL, V, VEC><<<grid, 32 * kBwdWarps, smem, stream>>>(
+      static_cast<const TL*>(logits), stat, ids, w, coef, gw, gl, T, E, K, static_cast<TL*>(out));
   return check_launch();
 }
 
@@ -329,12 +531,12 @@ template <typename TL, int V>
 int launch_backward(const void* logits, const float2* stat, const int32_t* ids, const float* w,
                     const float* coef, const float* gw, const float* gl, int T, int E, int K,
                     void* out, cudaStream_t stream) {
-  const size_t smem = static_cast<size_t>(E) * kWarps * 4;
-  const int want = (T + kWarps - 1) / kWarps;
-  const int grid = want < 148 * 8 ? want : 148 * 8;
-  router_backward_kernel<TL, V><<<grid, kThreads, smem, stream>>>(
-      static_cast<const TL*>(logits), stat, ids, w, coef, gw, gl, T, E, K, static_cast<TL*>(out));
-  return check_launch();
+  if constexpr (V * sizeof(TL) >= 4)
+    if (vec_rows<TL, V>(logits, out, E))
+      return launch_backward_as<TL, V, true>(logits, stat, ids, w, coef, gw, gl, T, E, K, out,
+                                             stream);
+  return launch_backward_as<TL, V, false>(logits, stat, ids, w, coef, gw, gl, T, E, K, out,
+                                          stream);
 }
 
 // Calls f<TL, V>() with TL by dtype and V the smallest power of two that holds ceil(E / 32).

@@ -7,8 +7,10 @@
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <algorithm>
 #include <array>
@@ -447,70 +449,107 @@ int logits_dtype(const torch::Tensor& t) {
   return dtype_code(t);
 }
 
-// Returns (topk_ids, topk_weights, tokens_per_expert, balance_loss, balance_counts, scratch,
-// row_stat, coef); the last two are what moe_router_backward takes.
+// Uninitialised tensor on `dev`: torch::empty without the dispatcher (the router makes six).
+torch::Tensor empty_on(const torch::Device& dev, at::IntArrayRef sizes, at::ScalarType dtype) {
+  return at::detail::empty_cuda(sizes, dtype, dev, c10::nullopt);
+}
+
+// Where the router keeps what its backward needs, behind the kernel's own scratch in one int32
+// tensor: (max, 1 / sum) per token, then one coefficient per expert.
+int64_t router_stat_at(int64_t T, int64_t E) {
+  const size_t sb = ggo_moe_router_scratch_bytes(T, static_cast<int>(E));
+  return static_cast<int64_t>((sb + 7) / 8 * 2);
+}
+float* router_stat(const torch::Tensor& scratch, int64_t T, int64_t E) {
+  return reinterpret_cast<float*>(scratch.data_ptr<int32_t>() + router_stat_at(T, E));
+}
+
+// topk_ids, topk_weights, tokens_per_expert, balance_loss, balance_counts, scratch
+using RouterOut = std::array<torch::Tensor, 6>;
+
+RouterOut router_forward(const torch::Tensor& logits, int64_t top_k,
+                         const c10::optional<torch::Tensor>& mask) {
+  const int64_t T = logits.size(0), E = logits.size(1);
+  const uint8_t* mp =
+      mask.has_value() ? reinterpret_cast<const uint8_t*>(mask->data_ptr<bool>()) : nullptr;
+  const auto dev = logits.device();
+  c10::cuda::CUDAGuard guard(dev);
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  auto ids = empty_on(dev, {T, top_k}, torch::kInt32);
+  auto w = empty_on(dev, {T, top_k}, torch::kFloat32);
+  auto tpe = empty_on(dev, {E}, torch::kInt64), kept = empty_on(dev, {E}, torch::kInt64);
+  auto loss = empty_on(dev, {}, torch::kFloat32);
+  auto scratch = empty_on(dev, {router_stat_at(T, E) + 2 * T + E}, torch::kInt32);
+  float* stat = router_stat(scratch, T, E);
+  check_status(ggo_moe_router(logits.data_ptr(), logits_dtype(logits), T, static_cast<int>(E),
+                              static_cast<int>(top_k), mp, ids.data_ptr<int32_t>(),
+                              w.data_ptr<float>(), tpe.data_ptr<int64_t>(),
+                              kept.data_ptr<int64_t>(), loss.data_ptr<float>(), stat, stat + 2 * T,
+                              scratch.data_ptr(), stream),
+               "MoE router");
+  return {ids, w, tpe, loss, kept, scratch};
+}
+
+// The routing as an autograd node. Its backward is a kernel of its own, not differentiable again: a
+// backward of the backward raises.
+struct RouterNode : public torch::autograd::Function<RouterNode> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
+                                                const torch::Tensor& logits, int64_t top_k,
+                                                const c10::optional<torch::Tensor>& mask) {
+    RouterOut o = router_forward(logits, top_k, mask);
+    ctx->save_for_backward({logits, o[0], o[1], o[5]});
+    ctx->mark_non_differentiable({o[0], o[2], o[4], o[5]});
+    ctx->set_materialize_grads(false);
+    return {o.begin(), o.end()};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    torch::Tensor gw = grads[1], gl = grads[3];
+    if (!gw.defined() && !gl.defined()) return {torch::Tensor(), torch::Tensor(), torch::Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    const torch::Tensor &logits = saved[0], &ids = saved[1], &w = saved[2], &scratch = saved[3];
+    torch::Tensor out;
+    {
+      at::NoGradGuard no_grad;
+      const int64_t T = logits.size(0), E = logits.size(1);
+      if (gw.defined()) gw = gw.contiguous();
+      c10::cuda::CUDAGuard guard(logits.device());
+      cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+      out = torch::empty_like(logits);
+      const float* stat = router_stat(scratch, T, E);
+      check_status(ggo_moe_router_backward(
+                       logits.data_ptr(), logits_dtype(logits), T, static_cast<int>(E),
+                       static_cast<int>(ids.size(1)), ids.data_ptr<int32_t>(),
+                       w.data_ptr<float>(), stat, stat + 2 * T,
+                       gw.defined() ? gw.data_ptr<float>() : nullptr,
+                       gl.defined() ? gl.data_ptr<float>() : nullptr, out.data_ptr(), stream),
+                   "MoE router backward");
+    }
+    if (at::GradMode::is_enabled()) {
+      auto refuse = std::make_shared<torch::autograd::DelayedError>(
+          "moe_router can be differentiated once only", 2);
+      out = (*refuse)({out, logits})[0];  // depends on the logits, by a way that is not recorded
+    }
+    return {out, torch::Tensor(), torch::Tensor()};
+  }
+};
+
 std::vector<torch::Tensor> moe_router(const torch::Tensor& logits, int64_t top_k,
                                       const c10::optional<torch::Tensor>& mask) {
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.is_contiguous(),
               "router_logits must be a contiguous 2D CUDA tensor");
+  logits_dtype(logits);  // raises for other types
   const int64_t T = logits.size(0), E = logits.size(1);
   TORCH_CHECK(E <= INT32_MAX && top_k > 0 && top_k <= E, "top_k must be in [1, num_experts]");
-  const uint8_t* mp = nullptr;
-  if (mask.has_value()) {
+  if (mask.has_value())
     TORCH_CHECK(mask->device() == logits.device() && mask->scalar_type() == torch::kBool &&
                     mask->dim() == 1 && mask->size(0) == T && mask->is_contiguous(),
                 "token_mask must be a contiguous bool tensor [T] on the logits' device");
-    mp = reinterpret_cast<const uint8_t*>(mask->data_ptr<bool>());
-  }
-  c10::cuda::CUDAGuard guard(logits.device());
-  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  const auto f32 = torch::TensorOptions().dtype(torch::kFloat32).device(logits.device());
-  const auto i32 = f32.dtype(torch::kInt32), i64 = f32.dtype(torch::kInt64);
-  auto ids = torch::empty({T, top_k}, i32);
-  auto w = torch::empty({T, top_k}, f32);
-  auto tpe = torch::empty({E}, i64), kept = torch::empty({E}, i64);
-  auto loss = torch::empty({}, f32), coef = torch::empty({E}, f32);
-  auto stat = torch::empty({T, 2}, f32);
-  const size_t sb = ggo_moe_router_scratch_bytes(T, static_cast<int>(E));
-  auto scratch = torch::empty({static_cast<int64_t>((sb + 3) / 4)}, i32);
-  check_status(ggo_moe_router(logits.data_ptr(), logits_dtype(logits), T, static_cast<int>(E),
-                              static_cast<int>(top_k), mp, ids.data_ptr<int32_t>(),
-                              w.data_ptr<float>(), tpe.data_ptr<int64_t>(),
-                              kept.data_ptr<int64_t>(), loss.data_ptr<float>(),
-                              stat.data_ptr<float>(), coef.data_ptr<float>(), scratch.data_ptr(),
-                              stream),
-               "MoE router");
-  return {ids, w, tpe, loss, kept, scratch, stat, coef};
-}
-
-torch::Tensor moe_router_backward(const torch::Tensor& logits, const torch::Tensor& ids,
-                                  const torch::Tensor& w, const torch::Tensor& stat,
-                                  const torch::Tensor& coef,
-                                  const c10::optional<torch::Tensor>& grad_w,
-                                  const c10::optional<torch::Tensor>& grad_loss) {
-  const float *gw = nullptr, *gl = nullptr;
-  if (grad_w.has_value()) {
-    TORCH_CHECK(grad_w->sizes() == w.sizes() && grad_w->scalar_type() == torch::kFloat32 &&
-                    grad_w->is_contiguous() && grad_w->device() == logits.device(),
-                "gradient of the weights: contiguous fp32 [T, top_k]");
-    gw = grad_w->data_ptr<float>();
-  }
-  if (grad_loss.has_value()) {
-    TORCH_CHECK(grad_loss->numel() == 1 && grad_loss->scalar_type() == torch::kFloat32 &&
-                    grad_loss->device() == logits.device(),
-                "gradient of the balance loss: one fp32");
-    gl = grad_loss->data_ptr<float>();
-  }
-  c10::cuda::CUDAGuard guard(logits.device());
-  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  auto out = torch::empty_like(logits);
-  check_status(ggo_moe_router_backward(
-                   logits.data_ptr(), logits_dtype(logits), logits.size(0),
-                   static_cast<int>(logits.size(1)), static_cast<int>(ids.size(1)),
-                   ids.data_ptr<int32_t>(), w.data_ptr<float>(), stat.data_ptr<float>(),
-                   coef.data_ptr<float>(), gw, gl, out.data_ptr(), stream),
-               "MoE router backward");
-  return out;
+  if (at::GradMode::is_enabled() && logits.requires_grad())
+    return RouterNode::apply(logits, top_k, mask);
+  RouterOut o = router_forward(logits, top_k, mask);
+  return {o.begin(), o.end()};
 }
 
 // Permute with INT8 quantisation: returns (q_sorted int8 [T*k, H], scale fp32 [T*k], slot_pos int32).
@@ -895,9 +934,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("tile_config") = 4, py::arg("sort_by_m") = true);
   m.def("moe_router", &moe_router, py::arg("router_logits"), py::arg("top_k"),
         py::arg("token_mask") = py::none());
-  m.def("moe_router_backward", &moe_router_backward, py::arg("router_logits"), py::arg("topk_ids"),
-        py::arg("topk_weights"), py::arg("row_stat"), py::arg("coef"), py::arg("grad_weights"),
-        py::arg("grad_loss"));
   m.def("moe_permute_int8", &moe_permute_int8, py::arg("hidden"), py::arg("topk_ids"),
         py::arg("scratch"), py::arg("num_experts"));
   m.def("moe_route", &moe_route, py::arg("router_logits"), py::arg("top_k"));

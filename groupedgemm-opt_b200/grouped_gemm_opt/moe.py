@@ -31,7 +31,6 @@ from typing import Callable, Optional
 
 import torch
 import torch.distributed as dist
-from torch.autograd.function import once_differentiable
 
 from grouped_gemm_opt.ops import TileConfig
 
@@ -106,31 +105,6 @@ class MoERouting:
     scratch: torch.Tensor            # the dispatch's offset table
 
 
-class _RouterFn(torch.autograd.Function):
-    """Forward: the routing kernel with the balance loss; backward: one kernel for the gradients that
-    reach the logits through the weights and through the loss."""
-
-    @staticmethod
-    def forward(ctx, logits, top_k, mask):
-        from grouped_gemm_opt._native import _C
-        ids, w, tpe, loss, kept, scratch, stat, coef = _C.moe_router(logits, top_k, mask)
-        ctx.save_for_backward(logits, ids, w, stat, coef)
-        ctx.mark_non_differentiable(ids, tpe, kept, scratch)
-        ctx.set_materialize_grads(False)
-        return ids, w, tpe, loss, kept, scratch
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, _ids, grad_w, _tpe, grad_loss, _kept, _scratch):
-        from grouped_gemm_opt._native import _C
-        if grad_w is None and grad_loss is None:
-            return None, None, None
-        logits, ids, w, stat, coef = ctx.saved_tensors
-        if grad_w is not None:
-            grad_w = grad_w.contiguous()
-        return (_C.moe_router_backward(logits, ids, w, stat, coef, grad_w, grad_loss), None, None)
-
-
 def moe_router(router_logits: torch.Tensor, top_k: int,
                token_mask: Optional[torch.Tensor] = None) -> MoERouting:
     """Top-k routing with the load-balance loss and per-expert counts, differentiable.
@@ -152,16 +126,18 @@ def moe_router(router_logits: torch.Tensor, top_k: int,
             in the loss, its gradient or ``balance_counts``. A token whose logits are all -inf
             has weights 0 and is not kept either. Without kept tokens the loss is 0.
 
-    Nothing synchronises; equal inputs give equal bits. Can be captured in a CUDA graph, the backward
-    together with the forward.
+    Nothing synchronises; equal inputs give equal bits. Differentiable once. Can be captured in a CUDA
+    graph, the backward together with the forward and by ``torch.autograd.grad``, while no eager
+    graph of the same leaf is alive (a rule of PyTorch's captures).
     """
+    from grouped_gemm_opt._native import _C
     assert router_logits.is_cuda and router_logits.dim() == 2
     assert 0 < top_k <= router_logits.size(1)
     if token_mask is not None:
         assert token_mask.dim() == 1 and token_mask.size(0) == router_logits.size(0), (
             "token_mask must have one entry per token")
         token_mask = token_mask.contiguous()
-    return MoERouting(*_RouterFn.apply(router_logits.contiguous(), top_k, token_mask))
+    return MoERouting(*_C.moe_router(router_logits.contiguous(), top_k, token_mask))
 
 
 def _routing_of(routing: MoERouting, router_logits, top_k):
@@ -659,8 +635,13 @@ def fused_moe_int8(hidden: torch.Tensor, router_logits: torch.Tensor, weights: M
     from grouped_gemm_opt._native import _C
     if timer is not None:
         timer.start()
-    ids, w, tpe, scratch = (_C.moe_route(router_logits, top_k) if routing is None
-                            else _routing_of(routing, router_logits, top_k))
+    if routing is None:
+        logits = router_logits.detach()
+        if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            logits = logits.float()
+        ids, w, tpe, _, _, scratch = _C.moe_router(logits.contiguous(), top_k, None)
+    else:
+        ids, w, tpe, scratch = _routing_of(routing, router_logits, top_k)
     _mark(timer, "route")
     xq, xsc, slot_pos = _C.moe_permute_int8(hidden.contiguous(), ids, scratch, E)
     _mark(timer, "dispatch")

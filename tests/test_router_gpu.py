@@ -314,3 +314,27 @@ def test_other_stream():
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(got.balance_loss, want.balance_loss)
     assert torch.equal(got.topk_ids, want.topk_ids)
+
+
+def test_second_derivatives_are_refused():
+    from grouped_gemm_opt import moe_router
+    leaf = torch.randn(20, 8, device=DEV, requires_grad=True)
+    g, = torch.autograd.grad(moe_router(leaf, 2).balance_loss, leaf, create_graph=True)
+    assert g.isfinite().all()
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(g.sum(), leaf)
+
+
+@pytest.mark.parametrize("E", [8, 40, 256, 1000])
+def test_nearly_equal_logits_are_ordered_exactly(E):
+    """fp32 logits that agree in their leading bits, among them equal ones: the order is that of all
+    their bits, ties to the lower index."""
+    from grouped_gemm_opt import moe_router
+    g = torch.Generator().manual_seed(E)
+    steps = torch.randint(0, 12, (300, E), generator=g).float()
+    for base in (1.0, -1.0, 100.0):
+        l = base * (1 + steps * 2.0 ** -22)
+        l[:50] = l[:50] + torch.randn(50, E, generator=g)
+        k = min(8, E)
+        want = torch.sort(l, dim=1, descending=True, stable=True)[1][:, :k]
+        assert torch.equal(moe_router(l.to(DEV), k).topk_ids.cpu().long(), want)
