@@ -139,6 +139,34 @@ def test_grouped_product(counts, n, k, dtype):
     check_device_errors(0)
 
 
+LONG = [([1], 256, 4096), ([16], 4096, 4096), ([64], 1000, 2064), ([3, 0, 30, 31], 264, 8192),
+         ([2] * 8, 14336, 4096), ([65], 128, 16384), ([200, 0, 90], 520, 3088), ([128], 256, 4096),
+         ([1000], 64, 9008), ([5] * 12, 1024, 1040)]
+
+
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("counts,n,k", LONG)
+def test_few_tiles_and_a_long_sum(counts, n, k, swiglu):
+    """Few output tiles and long sums, in every tile width; repeated calls agree to the bit."""
+    from grouped_gemm_opt import _C, check_device_errors
+    x, xs, w, ws = operands(counts, 2 * n if swiglu else n, k, seed=11)
+    dtype = torch.float16 if n % 16 else torch.bfloat16
+    if swiglu:
+        xs = xs * 4 / k ** 0.5
+        ref, g = swiglu_reference(counts, x, xs, w, ws)
+        tol = (2 * (2 + 1.2 * g.abs()) + 3 * (2 + g.abs()) + 8) * 2.0 ** -24
+    else:
+        ref, tol = reference(counts, x, xs, w, ws), 4 * 2.0 ** -24
+    dev = [t.to(DEV) for t in (x, xs, w, ws, torch.tensor(counts))]
+    for tc in (4, 0, 1):
+        out = _C.grouped_gemm_int8(*dev, swiglu, dtype, tc, True)
+        assert torch.all((out.cpu().double() - ref).abs() <=
+                         ref.abs() * (HALF_STEP[dtype] + tol) + LEAST[dtype])
+        for _ in range(10):
+            assert torch.equal(out, _C.grouped_gemm_int8(*dev, swiglu, dtype, tc, True))
+    check_device_errors(0)
+
+
 def test_longest_sum_does_not_wrap():
     """K = 131056 products of -128 with -128: 2147221504, just inside 32 bits, rounded to fp32."""
     from grouped_gemm_opt import grouped_gemm_opt_int8
