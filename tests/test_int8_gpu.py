@@ -53,6 +53,17 @@ def test_quantize_exact(rows, cols, dtype):
     check_quant(x)
 
 
+@pytest.mark.parametrize("cols", [32, 64, 80, 256, 272, 512, 528, 1008, 2032, 2064, 4080, 4112, 8192,
+                                  8208, 16368])
+def test_quantize_row_widths(cols):
+    """Both sides of every border between the forms for short, medium and long rows."""
+    g = torch.Generator().manual_seed(cols)
+    x = torch.randn(131, cols, generator=g).to(torch.bfloat16)
+    x[77, cols - 1] = 100.0  # the maximum in the last piece
+    x[130] = 0
+    check_quant(x)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_quantize_every_value(dtype):
     """Every finite value of the type in rows whose maximum is one of many: ties (x = max / 2 among
