@@ -66,7 +66,7 @@ enum DevError {
 };
 
 // 256 bytes of per-stream scratch. Must be zero before the first launch; each launch leaves the
-// two counters at zero again (the last CTA to finish resets them). `error` is sticky.
+// two counters at zero again (the last CTA to stop claiming tiles resets them). `error` is sticky.
 struct GgoWorkspace {
   int tile_counter;
   int done_counter;
@@ -219,9 +219,23 @@ __device__ __forceinline__ void build_segment_table(const GemmParams& p, uint8_t
     }
     __syncthreads();
   }
-  // Processing order: identity, or heaviest segment first (ties by index) via a bitonic sort of
-  // 64-bit keys held temporarily in the (still unused) operand tile buffers.
-  if (p.sort_by_m && nseg > 1) {
+  // Processing order: identity, or heaviest segment first (ties by index). Up to kThreads segments a
+  // thread each finds its segment's place by counting those before it (one barrier; 8 segments: 2300
+  // cycles less than the sort); more by a bitonic sort of 64-bit keys held temporarily in the (still
+  // unused) operand tile buffers.
+  if (p.sort_by_m && nseg > 1 && nseg <= kThreads) {
+    const int i = threadIdx.x;
+    if (i < nseg) {
+      const int mine = t_cnt[i];
+      int place = 0;
+#pragma unroll 8
+      for (int j = 0; j < nseg; ++j) {
+        const int c = t_cnt[j];
+        place += (c > mine || (c == mine && j < i)) ? 1 : 0;
+      }
+      t_order[place] = i;
+    }
+  } else if (p.sort_by_m && nseg > 1) {
     unsigned long long* keys = reinterpret_cast<unsigned long long*>(tiles);
     int n2 = 1;
     while (n2 < nseg) n2 <<= 1;
@@ -317,6 +331,16 @@ __device__ __forceinline__ void drain_armed_stages(uint64_t* full_bar, uint32_t 
     const long long t0 = clock64();
     while (!mbar_try_wait(a, par) && clock64() - t0 < limit) {
     }
+  }
+}
+
+// A producer that will claim no more tiles reports it, off the CTA's critical path; the last of the
+// grid returns the counters to zero for the next launch (no CTA claims after it).
+__device__ __forceinline__ void retire_claims(GgoWorkspace* ws) {
+  const int prev = atomicAdd(&ws->done_counter, 1);
+  if (prev == static_cast<int>(gridDim.x) - 1) {
+    atomicExch(&ws->tile_counter, 0);
+    atomicExch(&ws->done_counter, 0);
   }
 }
 
@@ -631,16 +655,36 @@ __device__ __forceinline__ OutT* output_row(const GemmParams& p, const TileInfo&
          static_cast<size_t>(o & 0x0fffffff) * p.n_out;
 }
 
+// Scales of a skinny tile: a lane's weight rows (one per half of the accumulator: two output columns,
+// or a gate and an up row) and, lane j, input rows j and 32 + j.
+template <int BN, int EPI>
+struct SkinnyScales {
+  float col[2], row[2];
+  __device__ __forceinline__ void load(const GemmParams& p, const TileInfo& info, int ew) {
+    const int lane = threadIdx.x & 31;
+    const float* scales = p.col_scale + static_cast<size_t>(info.seg % p.num_experts) * p.n_b;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = info.n0 + 32 * ew + lane + (epi_glu(EPI) ? 0 : 128 * h);
+      const bool ok = h < BN / 128 && c < p.n_out;
+      col[h] = ok ? __ldg(scales + c + (epi_glu(EPI) && h == 1 ? p.n_b / 2 : 0)) : 0.f;
+      const int r = 32 * h + lane;
+      row[h] = r < info.rows && info.row0 + r < p.rows ? __ldg(p.row_scale + info.row0 + r) : 0.f;
+    }
+  }
+};
+
 // Epilogue of a skinny (swapped-operand) tile. The accumulator is transposed: TMEM lane = weight
 // row, column = the tile's input row. The warp holding lanes [32 ew, 32 ew + 32) of weight half h
 // (TMEM columns [128 h, 128 h + 64)) owns output columns n0 + 128 h + 32 ew + lane (plain), or
 // n0 + 32 ew + lane with gate in half 0 and up in half 1 (SwiGLU). For every input row of the
-// tile the 32 lanes store 32 consecutive output columns (64 contiguous bytes). Scaled epilogues: a
-// lane's column scales stay with it, lane j of the warp reads the scale of input row j. All 32 lanes
-// must call it (tcgen05.ld is warp-collective).
+// tile the 32 lanes store 32 consecutive output columns (64 contiguous bytes), eight rows to a TMEM
+// read (a tile of one row that read and unrolled 32 spent 4500 cycles here, most of them fetching
+// instructions). All 32 lanes must call it (tcgen05.ld is warp-collective).
 template <int BN, int EPI, bool BF16, typename OutT, bool I8>
 __device__ __forceinline__ void store_skinny(uint32_t t_row, const GemmParams& p,
-                                             const TileInfo& info, int ew) {
+                                             const TileInfo& info, int ew,
+                                             const SkinnyScales<BN, EPI>& sk) {
   constexpr bool kScaled = EPI == kEpiScaled || EPI == kEpiScaledSwiGLU;
   const int lane = threadIdx.x & 31;
   constexpr int kHalves = epi_glu(EPI) ? 1 : BN / 128;
@@ -648,30 +692,22 @@ __device__ __forceinline__ void store_skinny(uint32_t t_row, const GemmParams& p
   for (int h = 0; h < kHalves; ++h) {
     const int col = info.n0 + 128 * h + 32 * ew + lane;
     const bool col_ok = col < p.n_out;
-    float cs = 0.f, cu = 0.f;
-    if (kScaled && col_ok) {
-      const float* scales = p.col_scale + static_cast<size_t>(info.seg % p.num_experts) * p.n_b;
-      cs = __ldg(scales + col);
-      if (epi_glu(EPI)) cu = __ldg(scales + p.n_b / 2 + col);
-    }
+    const float cs = h == 0 ? sk.col[0] : sk.col[1];
 #pragma unroll 1
-    for (int cb = 0; cb < info.rows; cb += 32) {
-      float row_scale = 0.f;
-      if (kScaled && cb + lane < info.rows && info.row0 + cb + lane < p.rows)
-        row_scale = __ldg(p.row_scale + info.row0 + cb + lane);
-      uint32_t v[32];
-      uint32_t u[32];
-      tmem_ld_32x32b_x32(t_row + 128 * h + cb, v);
-      if (epi_glu(EPI)) tmem_ld_32x32b_x32(t_row + 128 + cb, u);
+    for (int cb = 0; cb < info.rows; cb += 8) {
+      uint32_t v[8];
+      uint32_t u[8];
+      tmem_ld_32x32b_x8(t_row + 128 * h + cb, v);
+      if (epi_glu(EPI)) tmem_ld_32x32b_x8(t_row + 128 + cb, u);
       tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
+      for (int j = 0; j < 8; ++j) {
         const int r = cb + j;
         const bool ok = r < info.rows && info.row0 + r < p.rows;
         float y;
         if (kScaled) {
-          const float rs = __shfl_sync(0xffffffffu, row_scale, j);
-          y = epi_glu(EPI) ? scaled_silu_mul<I8>(v[j], u[j], rs, cs, cu)
+          const float rs = __shfl_sync(0xffffffffu, cb < 32 ? sk.row[0] : sk.row[1], r & 31);
+          y = epi_glu(EPI) ? scaled_silu_mul<I8>(v[j], u[j], rs, cs, sk.col[1])
                            : acc_to_float<I8>(v[j]) * rs * cs;
         } else {
           y = __uint_as_float(v[j]);
@@ -765,8 +801,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       int stage = 0, phase = 0, q = 0, qphase = 0;
       uint32_t armed = 0, armed_par = 0;  // stages whose loads were issued, and their parity
+      bool first = true;
       while (true) {
-        const int t = atomicAdd(&p.ws->tile_counter, 1);
+        // the first tile by block index, the others by claiming
+        const int t = first ? static_cast<int>(blockIdx.x)
+                            : static_cast<int>(gridDim.x) + atomicAdd(&p.ws->tile_counter, 1);
+        first = false;
         TileInfo info;
         info.rows = 0;
         if (t < total_tiles)
@@ -814,6 +854,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!ok) break;
       }
+      retire_claims(p.ws);
       if (guard->abort) drain_armed_stages<S>(full_bar, armed, armed_par, guard->limit);
     }
   } else if (warp == 1) {
@@ -899,14 +940,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&sche_bar[q]);
       if (++q == kSchedDepth) { q = 0; qphase ^= 1; }
       if (info.rows == 0) break;
-      if (!mbar_wait(&accf_bar[acc], aphase, guard, err, kDevTimeoutEpilogue)) break;
-      tc_fence_after();
       const int r_local = ew * 32 + lane;
       const bool row_ok = r_local < info.rows && info.row0 + r_local < p.rows;
+      constexpr bool kScaled = EPI == kEpiScaled || EPI == kEpiScaledSwiGLU;
+      // scales on their way while the MMAs run
+      SkinnyScales<BN, EPI> sk;
+      float rs = 1.f;
+      if (kSkinnyOk && kScaled && info.skinny)
+        sk.load(p, info, ew);
+      else if (kScaled && row_ok)
+        rs = __ldg(p.row_scale + info.row0 + r_local);
+      if (!mbar_wait(&accf_bar[acc], aphase, guard, err, kDevTimeoutEpilogue)) break;
+      tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + acc * BN;
       using OutT = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
       if (kSkinnyOk && info.skinny) {
-        store_skinny<BN, EPI, BF16, OutT, OP == kOpI8>(t_row, p, info, ew);
+        store_skinny<BN, EPI, BF16, OutT, OP == kOpI8>(t_row, p, info, ew, sk);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&acce_bar[acc]);
@@ -915,8 +964,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       OutT* out_row = output_row<OutT>(p, info, r_local, row_ok);
       const bool warp_tma = kTmaStoreOk && p.use_tma_store && ew * 32 + 32 <= info.rows;
-      constexpr bool kScaled = EPI == kEpiScaled || EPI == kEpiScaledSwiGLU;
-      const float rs = (kScaled && row_ok) ? __ldg(p.row_scale + info.row0 + r_local) : 1.f;
       // column scales: one per weight row, [E, n_b] (gate rows then up rows for SwiGLU)
       const float* cs_row =
           kScaled ? p.col_scale + static_cast<size_t>(info.seg % p.num_experts) * p.n_b : nullptr;
@@ -937,14 +984,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 2) {
     tc_fence_after();
     tmem_dealloc(tmem_base, kTmemCols);
-  }
-  if (threadIdx.x == 0) {
-    __threadfence();
-    const int prev = atomicAdd(&p.ws->done_counter, 1);
-    if (prev == static_cast<int>(gridDim.x) - 1) {
-      atomicExch(&p.ws->tile_counter, 0);
-      atomicExch(&p.ws->done_counter, 0);
-    }
   }
 }
 

@@ -167,11 +167,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       int stage = 0, phase = 0, q = 0, qphase = 0;
       uint32_t armed = 0, armed_par = 0;  // leader: stages armed, and their parity
+      bool first = true;
       while (true) {
         TileInfo info;
         bool stall_tile = false;  // test hook: this pair claimed tile 0
         if (leader) {
-          const int t = atomicAdd(&p.ws->tile_counter, 1);
+          // the first tile by pair index, the others by claiming
+          const int t = first ? static_cast<int>(blockIdx.x >> 1)
+                              : static_cast<int>(gridDim.x >> 1) + atomicAdd(&p.ws->tile_counter, 1);
+          first = false;
           stall_tile = t == 0;
           info.rows = 0;
           if (t < total_tiles)
@@ -244,6 +248,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         if (!ok) break;
       }
+      retire_claims(p.ws);
       // the leader's barriers count both CTAs' bytes; the final cluster barrier keeps the peer
       // resident until this drain is over
       if (leader && guard->abort) drain_armed_stages<S>(full_bar, armed, armed_par, guard->limit);
@@ -346,16 +351,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive_cluster(mapa_shared(&sche_bar[q], 0));
       if (++q == kSchedDepth) { q = 0; qphase ^= 1; }
       if (info.rows == 0) break;
-      if (!mbar_wait_cluster(&accf_bar[acc], aphase, guard, err, kDevTimeoutEpilogue)) break;
-      tc_fence_after();
       const int r_local = static_cast<int>(rank) * 128 + ew * 32 + lane;
       const bool row_ok = r_local < info.rows && info.row0 + r_local < p.rows;
+      constexpr bool kScaled = EPI == kEpiScaled || EPI == kEpiScaledSwiGLU;
+      const float rs = (kScaled && row_ok) ? __ldg(p.row_scale + info.row0 + r_local) : 1.f;
+      if (!mbar_wait_cluster(&accf_bar[acc], aphase, guard, err, kDevTimeoutEpilogue)) break;
+      tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + acc * kAccStride;
       OutT* out_row = output_row<OutT>(p, info, r_local, row_ok);
       const int wrow0 = static_cast<int>(rank) * 128 + ew * 32;
       const bool warp_tma = kTmaStoreOk && p.use_tma_store && wrow0 + 32 <= info.rows;
-      constexpr bool kScaled = EPI == kEpiScaled || EPI == kEpiScaledSwiGLU;
-      const float rs = (kScaled && row_ok) ? __ldg(p.row_scale + info.row0 + r_local) : 1.f;
       // column scales: one per weight row, [E, n_b] (gate rows then up rows for SwiGLU)
       const float* cs_row =
           kScaled ? p.col_scale + static_cast<size_t>(info.seg % p.num_experts) * p.n_b : nullptr;
@@ -383,14 +388,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 2) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, kTmemCols);
-  }
-  if (threadIdx.x == 0) {
-    __threadfence();
-    const int prev = atomicAdd(&p.ws->done_counter, 1);
-    if (prev == static_cast<int>(gridDim.x) - 1) {
-      atomicExch(&p.ws->tile_counter, 0);
-      atomicExch(&p.ws->done_counter, 0);
-    }
   }
 }
 
