@@ -243,12 +243,13 @@ __global__ void __launch_bounds__(256)
       const bool valid = i < nent;
       const unsigned vmask = __ballot_sync(kAll, valid);
       if (valid) {
-        const int id = ids[i];
+        // ids and offsets that do not belong together stay inside the buffers
+        const int id = min(max(ids[i], 0), E - 1);
         const unsigned peers = __match_any_sync(vmask, id);
         const int b = off[id];
         __syncwarp(vmask);
         if (lane == __ffs(peers) - 1) off[id] = b + __popc(peers);
-        const int ps = b + __popc(peers & ((1u << lane) - 1u));
+        const int ps = min(max(b + __popc(peers & ((1u << lane) - 1u)), 0), T * K - 1);
         pos[i] = ps;
         if (blockIdx.y == 0) slot_pos[static_cast<size_t>(t0) * K + i] = ps;
       }
@@ -325,9 +326,9 @@ int launch_permute(const void* x, int T, int H, int E, int K, const int32_t* ids
   const int nb = (T + kRouteTokens - 1) / kRouteTokens;
   const size_t smem = (static_cast<size_t>(E) + kRouteTokens * K) * 4;  // at most 6 KB
   const T16* xp = static_cast<const T16*>(x);
-  // Few tokens: all eight warps on one, so that every SM has a row. Else two, or one where a warp's
-  // registers hold the whole row. 16384 tokens x 4096 columns, two choices: 48 us (5.6 TB/s), 67 us with one warp
-  // per row that reads it twice and stores 8 bytes a lane.
+  // Few tokens: all eight warps on one, so that every SM has a row. Else as many as hold a row of that
+  // length in their registers. 16384 tokens x 4096 columns, two choices: 48 us (5.6 TB/s); 67 us with
+  // one warp per row that reads it twice and stores 8 bytes a lane.
   if (4 * nb <= 148)
     permute_int8_kernel<T16, 8, 2><<<dim3(nb, 32), 256, smem, stream>>>(
         xp, T, H, E, K, ids, offsets, q, scale, slot_pos);

@@ -47,7 +47,7 @@ bool capturing(cudaStream_t stream) {
 std::mutex g_ws_mu;
 std::map<std::pair<int, cudaStream_t>, torch::Tensor> g_ws;
 
-void* workspace_for(const torch::Device& dev, cudaStream_t stream) {
+void* workspace_for(const torch::Device& dev, cudaStream_t stream, bool in_capture) {
   std::lock_guard<std::mutex> lk(g_ws_mu);
   auto key = std::make_pair(static_cast<int>(dev.index()), stream);
   auto it = g_ws.find(key);
@@ -55,7 +55,7 @@ void* workspace_for(const torch::Device& dev, cudaStream_t stream) {
     const auto opts = torch::TensorOptions().dtype(torch::kUInt8).device(dev);
     const int64_t bytes = static_cast<int64_t>(ggo_workspace_size());
     torch::Tensor t;
-    if (capturing(stream)) {
+    if (in_capture) {
       // The first call on this stream is a captured one. The workspace outlives the graph and is
       // used outside it too, so it must neither come from the graph's memory pool nor be zeroed by
       // a node of the graph: make it on a stream that is not being captured, and wait for it.
@@ -74,23 +74,33 @@ void* workspace_for(const torch::Device& dev, cudaStream_t stream) {
   return it->second.data_ptr();
 }
 
+void* workspace_for(const torch::Device& dev, cudaStream_t stream) {
+  return workspace_for(dev, stream, capturing(stream));
+}
+
+// Stands for "any stream" among the keys of the workspaces: the one whose error word takes the errors
+// of captured calls, which may be replayed on any stream.
+cudaStream_t captured_key() { return reinterpret_cast<cudaStream_t>(&g_ws_mu); }
+
 // Workspace of one call. Eager calls share the stream's workspace (they run in stream order). A
 // captured call gets a zero-filled one of its own inside the graph, so that replays of several
-// graphs may overlap each other and eager calls; its device errors still go to the stream's.
+// graphs may overlap each other and eager calls; its device errors go to the device's word for
+// captured calls, which workspace_error reads too.
 struct CallWorkspace {
   torch::Tensor own;  // captured calls only
   void* ws = nullptr;
   int* err = nullptr;
 
   CallWorkspace(const torch::Device& dev, cudaStream_t stream) {
-    void* shared = workspace_for(dev, stream);
-    ws = shared;
-    err = ggo_workspace_error_word(shared);
-    if (capturing(stream)) {
-      own = torch::zeros({static_cast<int64_t>(ggo_workspace_size())},
-                         torch::TensorOptions().dtype(torch::kUInt8).device(dev));
-      ws = own.data_ptr();
+    if (!capturing(stream)) {
+      ws = workspace_for(dev, stream);
+      err = ggo_workspace_error_word(ws);
+      return;
     }
+    err = ggo_workspace_error_word(workspace_for(dev, captured_key(), true));
+    own = torch::zeros({static_cast<int64_t>(ggo_workspace_size())},
+                       torch::TensorOptions().dtype(torch::kUInt8).device(dev));
+    ws = own.data_ptr();
   }
 };
 
@@ -535,6 +545,21 @@ struct RouterNode : public torch::autograd::Function<RouterNode> {
   }
 };
 
+// A backward inside a graph capture ends on the stream of the leaf's accumulator node. While an eager
+// graph of the leaf is alive, that node is the eager one's, and the capture would be joined to a stream
+// outside it, which PyTorch does not survive: refuse before anything is recorded.
+void refuse_foreign_accumulator(const torch::Tensor& leaf) {
+  if (!leaf.is_leaf()) return;
+  const auto current = at::cuda::getCurrentCUDAStream(leaf.device().index());
+  if (!capturing(current)) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
+  if (!node) return;
+  const auto stream = node->stream();
+  TORCH_CHECK(!stream.has_value() || *stream == current.unwrap(),
+              "router_logits belong to an eager graph that is still alive: release it before "
+              "capturing a step over them");
+}
+
 std::vector<torch::Tensor> moe_router(const torch::Tensor& logits, int64_t top_k,
                                       const c10::optional<torch::Tensor>& mask) {
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.is_contiguous(),
@@ -546,8 +571,10 @@ std::vector<torch::Tensor> moe_router(const torch::Tensor& logits, int64_t top_k
     TORCH_CHECK(mask->device() == logits.device() && mask->scalar_type() == torch::kBool &&
                     mask->dim() == 1 && mask->size(0) == T && mask->is_contiguous(),
                 "token_mask must be a contiguous bool tensor [T] on the logits' device");
-  if (at::GradMode::is_enabled() && logits.requires_grad())
+  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    refuse_foreign_accumulator(logits);
     return RouterNode::apply(logits, top_k, mask);
+  }
   RouterOut o = router_forward(logits, top_k, mask);
   return {o.begin(), o.end()};
 }
@@ -646,15 +673,25 @@ torch::Tensor moe_combine(const torch::Tensor& y_sorted, const torch::Tensor& to
   return out;
 }
 
-// Reads and clears the device-side error word of the current stream's workspace (synchronises).
+// Reads and clears the device-side error word of the current stream's workspace, and that of captured
+// calls (synchronises).
 int64_t workspace_error(int64_t device) {
   c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const torch::Device dev(torch::kCUDA, static_cast<c10::DeviceIndex>(device));
   int code = 0;
-  const int st = ggo_workspace_error(
-      workspace_for(torch::Device(torch::kCUDA, static_cast<c10::DeviceIndex>(device)), stream),
-      stream, &code);
-  check_status(st, "workspace error read");
+  check_status(ggo_workspace_error(workspace_for(dev, stream), stream, &code),
+               "workspace error read");
+  if (code == 0) {  // and the word of captured calls, if there have been any
+    void* captured = nullptr;
+    {
+      std::lock_guard<std::mutex> lk(g_ws_mu);
+      auto it = g_ws.find(std::make_pair(static_cast<int>(device), captured_key()));
+      if (it != g_ws.end()) captured = it->second.data_ptr();
+    }
+    if (captured)
+      check_status(ggo_workspace_error(captured, stream, &code), "workspace error read");
+  }
   return code;
 }
 

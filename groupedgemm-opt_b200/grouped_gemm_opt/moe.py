@@ -127,8 +127,9 @@ def moe_router(router_logits: torch.Tensor, top_k: int,
             has weights 0 and is not kept either. Without kept tokens the loss is 0.
 
     Nothing synchronises; equal inputs give equal bits. Differentiable once. Can be captured in a CUDA
-    graph, the backward together with the forward and by ``torch.autograd.grad``, while no eager
-    graph of the same leaf is alive (a rule of PyTorch's captures).
+    graph, the backward together with the forward and by ``torch.autograd.grad``. That needs every
+    eager graph of the same leaves to be gone (PyTorch ends the process otherwise); for logits that
+    are themselves such a leaf the call is refused.
     """
     from grouped_gemm_opt._native import _C
     assert router_logits.is_cuda and router_logits.dim() == 2
@@ -334,8 +335,8 @@ def fused_moe(
         ep_buffers: EPBuffers of `ep_group`: selects the fused peer-memory path (dispatch and
             result scatter over NVLink inside the kernels) instead of NCCL all-to-alls.
         timer: a StageEvents that records a CUDA event after every stage (device timing).
-        routing: the result of ``moe_router(router_logits, top_k)``: the layer uses it instead of
-            routing again.
+        routing: the result of ``moe_router(router_logits, top_k)``, unchanged: the layer uses it
+            instead of routing again.
 
     Returns: [T, H] = sum_j w[t,j] * down(silu(gate(x_t)) * up(x_t)) for the top-k experts.
     """

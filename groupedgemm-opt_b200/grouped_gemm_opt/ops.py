@@ -106,7 +106,8 @@ def grouped_gemm_opt(
 
 def check_device_errors(device: int = 0) -> None:
     """Synchronises and raises RuntimeError if a kernel on the current stream recorded an error
-    (count mismatch with GPU counts, negative count, or an expired bounded wait)."""
+    (count mismatch with GPU counts, negative count, or an expired bounded wait), or an INT8 product
+    replayed from a CUDA graph did."""
     code = int(_C.workspace_error(device))
     if code:
         raise RuntimeError(f"grouped_gemm_opt device error code {code}")

@@ -413,3 +413,69 @@ def test_host_counts_are_refused_in_a_capture():
     with torch.cuda.graph(g):
         with pytest.raises(RuntimeError, match="captured"):
             grouped_gemm_opt_int8(x, xs, w, ws, tpe)
+
+
+def test_errors_of_a_replayed_call_are_reported():
+    """Counts that stop matching between capture and replay: the replay records it, wherever it runs."""
+    from grouped_gemm_opt import check_device_errors, grouped_gemm_opt_int8
+    x, xs, w, ws = (t.to(DEV) for t in operands([20, 12], 64, 64))
+    tpe = torch.tensor([20, 12], device=DEV)
+    want = grouped_gemm_opt_int8(x, xs, w, ws, tpe)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = grouped_gemm_opt_int8(x, xs, w, ws, tpe)
+    g.replay()
+    check_device_errors(0)
+    assert torch.equal(out, want)
+    tpe[1] = 11
+    g.replay()
+    with pytest.raises(RuntimeError):
+        check_device_errors(0)
+    tpe[1] = 12
+    g.replay()
+    check_device_errors(0)
+    assert torch.equal(out, want)
+
+
+def test_nan_token_stays_alone_in_the_layer():
+    from grouped_gemm_opt import fused_moe_int8, quantize_moe_weights_int8
+    x, logits, wgu, wd = layer_inputs(90, 64, 128, 4, torch.bfloat16)
+    qw = quantize_moe_weights_int8(wgu.to(DEV), wd.to(DEV))
+    xd, ld = x.to(DEV), logits.to(DEV)
+    want = fused_moe_int8(xd, ld, qw, 2)
+    xd[17, 3] = float("nan")
+    xd[40, 9] = float("inf")
+    out = fused_moe_int8(xd, ld, qw, 2)
+    hit = torch.zeros(90, dtype=torch.bool, device=DEV)
+    hit[[17, 40]] = True
+    assert out[hit].isnan().all() and torch.equal(out[~hit], want[~hit])
+
+
+def test_layer_with_logits_of_other_types():
+    """The layer routes on whatever float type the logits have, as the others do."""
+    from grouped_gemm_opt import fused_moe_int8, quantize_moe_weights_int8
+    x, logits, wgu, wd = layer_inputs(70, 64, 128, 4, torch.bfloat16)
+    qw = quantize_moe_weights_int8(wgu.to(DEV), wd.to(DEV))
+    half = logits.to(torch.float16)
+    want = fused_moe_int8(x.to(DEV), half.float().to(DEV), qw, 2)
+    for l in (half, half.double(), half.float().t().contiguous().t()):
+        assert torch.equal(fused_moe_int8(x.to(DEV), l.to(DEV), qw, 2), want)
+    strided = x.to(DEV).t().contiguous().t()
+    assert torch.equal(fused_moe_int8(strided, half.to(DEV), qw, 2), want)
+
+
+def test_products_on_two_streams_at_once():
+    from grouped_gemm_opt import check_device_errors, grouped_gemm_opt_int8
+    counts = [500, 0, 900, 33]
+    dev = [t.to(DEV) for t in operands(counts, 2048, 1024)] + [torch.tensor(counts, device=DEV)]
+    want = grouped_gemm_opt_int8(*dev)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 3]):
+            outs.append(grouped_gemm_opt_int8(*dev))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    check_device_errors(0)

@@ -126,3 +126,48 @@ def test_routing_of_another_shape_is_refused():
         fused_moe(x, torch.randn(4, 8), wgu, wd, 3, routing=r)
     with pytest.raises(AssertionError, match="routing is for"):
         fused_moe(torch.randn(5, 16), torch.randn(5, 8), wgu, wd, 2, routing=r)
+
+
+def test_given_routing_replaces_the_route_stage():
+    """fused_moe with a routing runs the other stages on it and does not route again."""
+    from grouped_gemm_opt.moe import MoEOps, MoERouting, fused_moe
+    T, H, F, E, k = 6, 8, 16, 4, 2
+    g = torch.Generator().manual_seed(0)
+    x, logits = torch.randn(T, H, generator=g), torch.randn(T, E, generator=g)
+    wgu, wd = torch.randn(E, 2 * F, H, generator=g), torch.randn(E, H, F, generator=g)
+    ids = torch.sort(logits, dim=1, descending=True)[1][:, :k].to(torch.int32)
+    w = torch.softmax(logits.gather(1, ids.long()), 1).requires_grad_(True)
+    tpe = torch.bincount(ids.flatten().long(), minlength=E)
+    r = MoERouting(ids, w, tpe, torch.tensor(1.0), tpe, torch.zeros(8, dtype=torch.int32))
+    seen = []
+
+    def permute(xs, i, scratch, experts):
+        assert i is ids and scratch is r.scratch and experts == E
+        order = torch.sort(ids.flatten(), stable=True)[1]
+        pos = torch.empty(T * k, dtype=torch.int64)
+        pos[order] = torch.arange(T * k)
+        return xs[order // k], None, pos
+
+    def no_route(*_):
+        raise AssertionError("routed again")
+
+    def experts(f):
+        def stage(rows, weights, counts, n, sort):
+            assert counts is tpe
+            return torch.cat([f(a, weights[e]) for e, a in enumerate(rows.split(counts.tolist()))])
+        return stage
+
+    def glu(a, m):
+        gate, up = (a @ m.t()).chunk(2, 1)
+        return torch.nn.functional.silu(gate) * up
+
+    def combine(y, weights, pos):
+        assert not weights.requires_grad
+        seen.append(True)
+        return (y[pos].reshape(T, k, H) * weights[:, :, None]).sum(1)
+
+    ops = MoEOps(no_route, permute, experts(glu), experts(lambda a, m: a @ m.t()), combine)
+    out = fused_moe(x, logits, wgu, wd, k, ops=ops, routing=r)
+    want = sum(w.detach()[:, j, None] * torch.stack(
+        [wd[ids[t, j]] @ glu(x[t][None], wgu[ids[t, j]])[0] for t in range(T)]) for j in range(k))
+    assert seen and torch.allclose(out, want, rtol=1e-4, atol=1e-4)

@@ -338,3 +338,21 @@ def test_nearly_equal_logits_are_ordered_exactly(E):
         k = min(8, E)
         want = torch.sort(l, dim=1, descending=True, stable=True)[1][:, :k]
         assert torch.equal(moe_router(l.to(DEV), k).topk_ids.cpu().long(), want)
+
+
+def test_capture_over_a_live_eager_graph_is_refused():
+    from grouped_gemm_opt import moe_router
+    leaf = torch.randn(40, 16, device=DEV, requires_grad=True)
+    alive = moe_router(leaf, 2)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match="still alive"):
+            moe_router(leaf, 2)
+        with torch.no_grad():
+            moe_router(leaf, 2)  # without a gradient there is nothing to refuse
+    alive.balance_loss.backward()
+    assert leaf.grad.isfinite().all()
+    del alive
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        moe_router(leaf, 2)
