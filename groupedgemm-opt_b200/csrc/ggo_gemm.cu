@@ -140,7 +140,7 @@ int make_b_map(CUtensorMap* m, const void* b, int64_t b_rows, const GemmParams& 
   return make_map(m, b, b_rows, q.k, bf16, box_rows);
 }
 
-template <int BN, int EPI, bool BF16, bool BMN = false, int OP = kOp16>
+template <int BN, int EPI, bool BF16, bool BMN = false, int OP = kOp16, bool THIN = false>
 int launch(const void* a, const void* b, int64_t b_rows, const GemmParams& p, int dev,
            cudaStream_t stream) {
   CUtensorMap ma, mb, mc, mas;
@@ -150,7 +150,7 @@ int launch(const void* a, const void* b, int64_t b_rows, const GemmParams& p, in
     if (int st = make_map_byte(&ma, a, q.rows, q.k, kBM)) return st;
     if (int st = make_map_byte(&mb, b, b_rows, q.k, 128)) return st;
     if (OP == kOpE4M3) q.skinny_max = 0;
-    if (q.skinny_max > 0)
+    if (THIN || q.skinny_max > 0)
       if (int st = make_map_byte(&mas, a, q.rows, q.k, kSkinnyRows)) return st;
   } else {
     if (int st = make_map(&ma, a, q.rows, q.k, BF16, kBM)) return st;
@@ -162,8 +162,8 @@ int launch(const void* a, const void* b, int64_t b_rows, const GemmParams& p, in
     }
   }
   if (int st = make_out_map(&mc, &q, BF16)) return st;
-  auto kern = grouped_gemm_kernel<BN, EPI, BF16, BMN, OP>;
-  constexpr int smem = SmemLayout<BN>::kTotal;
+  auto kern = grouped_gemm_kernel<BN, EPI, BF16, BMN, OP, THIN>;
+  constexpr int smem = SmemLayout<BN, THIN>::kTotal;
   int sms = 0;
   if (int st = kernel_setup(kern, smem, dev, false, &sms)) return st;
   constexpr int out_bn = epi_glu(EPI) ? BN / 2 : BN;
@@ -346,6 +346,14 @@ int launch_scaled(const void* input, const void* weights, int64_t b_rows, GemmPa
     const int st = launch_pair<256, EPI, BF16, false, OP>(input, weights, b_rows, pp, dev, stream);
     if (st || !split) return st;
     p.split_mode = 2;
+  }
+  if constexpr (OP == kOpI8) {
+    if (p.rows <= kSkinnyRows && p.skinny_max == kSkinnyRows) {
+      if constexpr (!epi_glu(EPI))
+        if (bn == 128)
+          return launch<128, EPI, BF16, false, OP, true>(input, weights, b_rows, p, dev, stream);
+      return launch<256, EPI, BF16, false, OP, true>(input, weights, b_rows, p, dev, stream);
+    }
   }
   if constexpr (OP == kOpI8 && !epi_glu(EPI))
     if (bn == 128) return launch<128, EPI, BF16, false, OP>(input, weights, b_rows, p, dev, stream);

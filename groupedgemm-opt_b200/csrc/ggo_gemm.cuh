@@ -13,7 +13,7 @@
 //  * No per-group tensor maps: all experts share K, so one 2D TMA map over in[T,K] and one over
 //    W viewed as [E*N, K] serve every segment. Rows of a tile past its segment's end are loaded
 //    (they belong to the next segment or are TMA zero-fill) and masked at the store.
-//  * Warp specialisation: warp 0 = TMA producer, warp 1 = single-thread tcgen05.mma issuer,
+//  * Warp specialisation: warp 0 = TMA producer, warp 1 = tcgen05.mma issuer (one elected thread),
 //    warp 2 = TMEM allocator, warps 4..7 = epilogue (TMEM -> registers -> shared-memory staging
 //    -> TMA stores; masked 16-byte stores where a warp's rows cross a segment boundary).
 //    Two TMEM accumulators let the epilogue of tile i overlap the MMAs of tile i+1.
@@ -42,6 +42,7 @@ constexpr int kUmmaK = 16;        // K per tcgen05.mma kind::f16
 constexpr int kMaxSegments = 1024;
 constexpr int kSchedDepth = 4;
 constexpr int kThreads = 256;
+constexpr int kSkinnyRows = 64;   // rows of the input box a skinny tile loads (its row limit)
 
 // Operand element types of the GEMM kernels (template parameter OP).
 enum OpKind { kOp16 = 0, kOpE4M3 = 1, kOpI8 = 2 };
@@ -111,7 +112,6 @@ struct GemmParams {
   int* err;  // where device errors are recorded (first one wins): &ws->error unless given apart
 };
 
-constexpr int kSkinnyRows = 64;  // rows of the input box a skinny tile loads (its row limit)
 
 struct TileInfo {
   int row0;    // first input row of the tile
@@ -124,14 +124,17 @@ struct TileInfo {
   int pad;
 };
 
-template <int BN>
+// THIN: a launch of at most kSkinnyRows rows, whose tiles are all skinny: the A slot holds the skinny
+// box only, nothing is staged for TMA stores, and the room goes to more stages: 128 or 160 KB of weights
+// in flight instead of 96 or 128.
+template <int BN, bool THIN = false>
 struct SmemLayout {
-  static constexpr int kStages = (BN == 256) ? 4 : 6;
-  static constexpr int kABytes = kBM * kBK * 2;   // 16 KB
+  static constexpr int kStages = THIN ? (BN == 256 ? 5 : 8) : (BN == 256 ? 4 : 6);
+  static constexpr int kABytes = (THIN ? kSkinnyRows : kBM) * kBK * 2;  // 8 or 16 KB
   static constexpr int kBBytes = BN * kBK * 2;    // 32 KB or 16 KB
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kTileBytes = kStages * kStageBytes;
-  static constexpr int kStagingBytes = 4 * 4096;  // TMA-store staging, 4 KB per epilogue warp
+  static constexpr int kStagingBytes = THIN ? 0 : 4 * 4096;  // TMA-store staging, 4 KB per warp
   static constexpr int kTableBytes = 4 * kMaxSegments * 4 + 16;
   static constexpr int kMiscBytes = 1024;
   static constexpr int kTotal =
@@ -720,19 +723,20 @@ __device__ __forceinline__ void store_skinny(uint32_t t_row, const GemmParams& p
   }
 }
 
-template <int BN, int EPI, bool BF16, bool BMN = false, int OP = kOp16>
+template <int BN, int EPI, bool BF16, bool BMN = false, int OP = kOp16, bool THIN = false>
 __global__ void __launch_bounds__(kThreads, 1)
     grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA,
                         const __grid_constant__ CUtensorMap tmB,
                         const __grid_constant__ CUtensorMap tmC,
                         const __grid_constant__ CUtensorMap tmAs, const GemmParams p) {
-  using L = SmemLayout<BN>;
+  using L = SmemLayout<BN, THIN>;
   constexpr int S = L::kStages;
   constexpr int kTmemCols = 2 * BN;             // two accumulators
   constexpr int kOutBN = epi_glu(EPI) ? BN / 2 : BN;
   constexpr bool kTmaStoreOk = kOutBN % 64 == 0;  // output boxes are 64 columns wide
   // skinny tiles: tmAs is the input map with kSkinnyRows-row boxes
   constexpr bool kSkinnyOk = !BMN && OP != kOpE4M3;
+  static_assert(!THIN || kSkinnyOk, "thin launches are skinny ones");
   constexpr int kSkinnyABytes = kSkinnyRows * kBK * 2;
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -798,39 +802,47 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     // -------------------------------------------------------------- TMA producer
-    if (lane == 0) {
+    {
+      const bool issuer = elect_one();
+      const int issuer_lane = __ffs(__ballot_sync(0xffffffffu, issuer)) - 1;
       int stage = 0, phase = 0, q = 0, qphase = 0;
       uint32_t armed = 0, armed_par = 0;  // stages whose loads were issued, and their parity
       bool first = true;
       while (true) {
         // the first tile by block index, the others by claiming
-        const int t = first ? static_cast<int>(blockIdx.x)
-                            : static_cast<int>(gridDim.x) + atomicAdd(&p.ws->tile_counter, 1);
+        int t = static_cast<int>(blockIdx.x);
+        if (!first) {
+          if (issuer) t = static_cast<int>(gridDim.x) + atomicAdd(&p.ws->tile_counter, 1);
+          t = __shfl_sync(0xffffffffu, t, issuer_lane);
+        }
         first = false;
         TileInfo info;
         info.rows = 0;
         if (t < total_tiles)
           info = decode_tile<kBM, kOutBN, EPI, 128, BMN>(interleave_tile(t, heavy_tiles, total_tiles),
                                                         p, t_cnt, t_rowoff, t_order, t_tileoff);
-        info.skinny = (kSkinnyOk && info.rows > 0 && info.rows <= p.skinny_max) ? 1 : 0;
-        if (!mbar_wait(&sche_bar[q], qphase ^ 1, guard, err, kDevTimeoutProducer)) break;
-        ring[q] = info;
-        mbar_arrive(&schf_bar[q]);
+        info.skinny =
+            (kSkinnyOk && info.rows > 0 && (THIN || info.rows <= p.skinny_max)) ? 1 : 0;
+        if (!mbar_wait_warp(&sche_bar[q], qphase ^ 1, guard, err, kDevTimeoutProducer)) break;
+        if (issuer) {
+          ring[q] = info;
+          mbar_arrive(&schf_bar[q]);
+        }
         if (++q == kSchedDepth) { q = 0; qphase ^= 1; }
         if (info.rows == 0) break;
         bool ok = true;
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(&empty_bar[stage], phase ^ 1, guard, err, kDevTimeoutProducer)) {
+          if (!mbar_wait_warp(&empty_bar[stage], phase ^ 1, guard, err, kDevTimeoutProducer)) {
             ok = false;
             break;
           }
           // test hook: the CTA that claimed tile 0 leaves that tile's first stage unarmed, so its
           // MMA's bounded wait expires
           const bool skip = p.inject_stall && t == 0 && kb == 0;
-          if (!skip) {
+          if (!skip && issuer) {
             uint8_t* a_dst = tiles + stage * L::kStageBytes;
             uint8_t* b_dst = a_dst + L::kABytes;
-            if (kSkinnyOk && info.skinny) {  // only the tile's first kSkinnyRows input rows
+            if (THIN || (kSkinnyOk && info.skinny)) {  // only the tile's first kSkinnyRows input rows
               mbar_arrive_expect_tx(&full_bar[stage], kSkinnyABytes + L::kBBytes);
               tma_load_2d(a_dst, &tmAs, &full_bar[stage], kb * kStageK, info.row0);
             } else {
@@ -847,6 +859,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (BN == 256)
                 tma_load_2d(b_dst + 128 * 128, &tmB, &full_bar[stage], kb * kStageK, info.brow1);
             }
+          }
+          if (!skip) {
             armed |= 1u << stage;
             armed_par = (armed_par & ~(1u << stage)) | (static_cast<uint32_t>(phase) << stage);
           }
@@ -854,34 +868,36 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!ok) break;
       }
-      retire_claims(p.ws);
+      if (issuer) retire_claims(p.ws);
       if (guard->abort) drain_armed_stages<S>(full_bar, armed, armed_par, guard->limit);
     }
   } else if (warp == 1) {
     // -------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
+    {
+      const bool issuer = elect_one();
       // e4m3 operands are format 0 of kind::f8f6f4, the same bits as f16 in kind::f16
       constexpr uint32_t idesc = OP == kOpI8 ? idesc_i8(kBM, BN)
                                              : idesc_f16(kBM, BN, OP == kOp16 && BF16, BMN);
       int stage = 0, phase = 0, q = 0, qphase = 0, acc = 0, aphase = 0;
       const uint32_t tiles_addr = smem_u32(tiles);
       while (true) {
-        if (!mbar_wait(&schf_bar[q], qphase, guard, err, kDevTimeoutMma)) break;
+        if (!mbar_wait_warp(&schf_bar[q], qphase, guard, err, kDevTimeoutMma)) break;
         const bool valid = ring[q].rows > 0;
-        const bool skinny = kSkinnyOk && ring[q].skinny;
+        const bool skinny = THIN || (kSkinnyOk && ring[q].skinny);
         // skinny: M = 128 weight rows per MMA, N = the tile's rows rounded up to 16
         const int n_s = (ring[q].rows + 15) & ~15;
         const uint32_t idesc_s = OP == kOpI8 ? idesc_i8(kBM, n_s)
                                              : idesc_f16(kBM, n_s, BF16, false);
-        mbar_arrive(&sche_bar[q]);
+        __syncwarp();
+        if (issuer) mbar_arrive(&sche_bar[q]);
         if (++q == kSchedDepth) { q = 0; qphase ^= 1; }
         if (!valid) break;
-        if (!mbar_wait(&acce_bar[acc], aphase ^ 1, guard, err, kDevTimeoutMma)) break;
+        if (!mbar_wait_warp(&acce_bar[acc], aphase ^ 1, guard, err, kDevTimeoutMma)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
         bool ok = true;
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(&full_bar[stage], phase, guard, err, kDevTimeoutMma)) {
+          if (!mbar_wait_warp(&full_bar[stage], phase, guard, err, kDevTimeoutMma)) {
             ok = false;
             break;
           }
@@ -893,39 +909,41 @@ __global__ void __launch_bounds__(kThreads, 1)
           // per 16-element K step: A (K-major) advances 32 B inside its swizzle atom; a K-major
           // B likewise, an MN-major B by 16 rows of 128 B (two 8-row atoms)
           constexpr uint64_t kBStep = BMN ? (2048 >> 4) : 2;
-          if (kSkinnyOk && skinny) {
+          if (THIN || (kSkinnyOk && skinny)) {
             // weights (the B slot, 128 rows per half) as the M-side operand, the tile's rows
             // (the A slot) as the N side; half h accumulates into TMEM columns [128 h, ...)
+            if (issuer) {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
+              for (int kk = 0; kk < 4; ++kk) {
 #pragma unroll
-              for (int h = 0; h < BN / 128; ++h) {
-                const uint64_t wdesc =
-                    sdesc_sw128_kmajor(a_addr + L::kABytes + h * 16384) + 2 * kk;
-                if (OP == kOpI8)
-                  mma_i8_ss(d_tmem + 128 * h, wdesc, adesc + 2 * kk, idesc_s, (kb | kk) != 0);
-                else
-                  mma_f16_ss(d_tmem + 128 * h, wdesc, adesc + 2 * kk, idesc_s, (kb | kk) != 0);
+                for (int h = 0; h < BN / 128; ++h) {
+                  const uint64_t wdesc =
+                      sdesc_sw128_kmajor(a_addr + L::kABytes + h * 16384) + 2 * kk;
+                  if (OP == kOpI8)
+                    mma_i8_ss(d_tmem + 128 * h, wdesc, adesc + 2 * kk, idesc_s, (kb | kk) != 0);
+                  else
+                    mma_f16_ss(d_tmem + 128 * h, wdesc, adesc + 2 * kk, idesc_s, (kb | kk) != 0);
+                }
               }
+              mma_commit(&empty_bar[stage]);
+            }
+          } else if (issuer) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {  // four 32-byte K steps per 128-byte stage row
+              if (OP == kOpI8)
+                mma_i8_ss(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
+              else if (OP == kOpE4M3)
+                mma_f8_ss(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
+              else
+                mma_f16_ss(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
             }
             mma_commit(&empty_bar[stage]);
-            if (++stage == S) { stage = 0; phase ^= 1; }
-            continue;
           }
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {  // four 32-byte K steps per 128-byte stage row
-            if (OP == kOpI8)
-              mma_i8_ss(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
-            else if (OP == kOpE4M3)
-              mma_f8_ss(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
-            else
-              mma_f16_ss(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
-          }
-          mma_commit(&empty_bar[stage]);
+          __syncwarp();
           if (++stage == S) { stage = 0; phase ^= 1; }
         }
         if (!ok) break;
-        mma_commit(&accf_bar[acc]);
+        if (issuer) mma_commit(&accf_bar[acc]);
         if (++acc == 2) { acc = 0; aphase ^= 1; }
       }
     }
@@ -946,7 +964,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // scales on their way while the MMAs run
       SkinnyScales<BN, EPI> sk;
       float rs = 1.f;
-      if (kSkinnyOk && kScaled && info.skinny)
+      if (kSkinnyOk && kScaled && (THIN || info.skinny))
         sk.load(p, info, ew);
       else if (kScaled && row_ok)
         rs = __ldg(p.row_scale + info.row0 + r_local);
@@ -954,7 +972,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + acc * BN;
       using OutT = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-      if (kSkinnyOk && info.skinny) {
+      if (THIN || (kSkinnyOk && info.skinny)) {
         store_skinny<BN, EPI, BF16, OutT, OP == kOpI8>(t_row, p, info, ew, sk);
         tc_fence_before();
         __syncwarp();

@@ -164,7 +164,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     // -------------------------------------------------------------- TMA producers (both CTAs)
-    if (lane == 0) {
+    {
+      const bool issuer = elect_one();
+      const int issuer_lane = __ffs(__ballot_sync(0xffffffffu, issuer)) - 1;
       int stage = 0, phase = 0, q = 0, qphase = 0;
       uint32_t armed = 0, armed_par = 0;  // leader: stages armed, and their parity
       bool first = true;
@@ -173,8 +175,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         bool stall_tile = false;  // test hook: this pair claimed tile 0
         if (leader) {
           // the first tile by pair index, the others by claiming
-          const int t = first ? static_cast<int>(blockIdx.x >> 1)
-                              : static_cast<int>(gridDim.x >> 1) + atomicAdd(&p.ws->tile_counter, 1);
+          int t = static_cast<int>(blockIdx.x >> 1);
+          if (!first) {
+            if (issuer) t = static_cast<int>(gridDim.x >> 1) + atomicAdd(&p.ws->tile_counter, 1);
+            t = __shfl_sync(0xffffffffu, t, issuer_lane);
+          }
           first = false;
           stall_tile = t == 0;
           info.rows = 0;
@@ -182,19 +187,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             info = decode_tile<kTileM, kOutBN, EPI, BN / 2, BMN>(
                 interleave_tile(t, heavy_tiles, total_tiles), p, t_cnt, t_rowoff, t_order,
                                                                t_tileoff);
-          if (!mbar_wait_cluster(&sche_bar[q], qphase ^ 1, guard, err, kDevTimeoutProducer))
+          if (!mbar_wait_cluster_warp(&sche_bar[q], qphase ^ 1, guard, err, kDevTimeoutProducer))
             break;
-          ring[q] = info;
-          const uint32_t pr = mapa_shared(&ring[q], 1);
-          st_cluster_v4(pr, info.row0, info.rows, info.n0, info.brow0);
-          st_cluster_v4(pr + 16, info.brow1, info.seg, 0, 0);
-          mbar_arrive(&schf_bar[q]);
-          mbar_arrive_cluster(mapa_shared(&schf_bar[q], 1));
+          if (issuer) {
+            ring[q] = info;
+            const uint32_t pr = mapa_shared(&ring[q], 1);
+            st_cluster_v4(pr, info.row0, info.rows, info.n0, info.brow0);
+            st_cluster_v4(pr + 16, info.brow1, info.seg, 0, 0);
+            mbar_arrive(&schf_bar[q]);
+            mbar_arrive_cluster(mapa_shared(&schf_bar[q], 1));
+          }
         } else {
-          if (!mbar_wait_cluster(&schf_bar[q], qphase, guard, err, kDevTimeoutProducer))
+          if (!mbar_wait_cluster_warp(&schf_bar[q], qphase, guard, err, kDevTimeoutProducer))
             break;
           info = ring[q];
-          mbar_arrive_cluster(mapa_shared(&sche_bar[q], 0));
+          __syncwarp();
+          if (issuer) mbar_arrive_cluster(mapa_shared(&sche_bar[q], 0));
         }
         if (++q == kSchedDepth) { q = 0; qphase ^= 1; }
         if (info.rows == 0) break;
@@ -202,21 +210,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int b_row = leader ? info.brow0 : info.brow1;
         bool ok = true;
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait_cluster(&empty_bar[stage], phase ^ 1, guard, err,
+          if (!mbar_wait_cluster_warp(&empty_bar[stage], phase ^ 1, guard, err,
                                  kDevTimeoutProducer)) {
             ok = false;
             break;
           }
           // test hook: the leader of the pair that claimed tile 0 leaves its first stage unarmed
           const bool skip = p.inject_stall && stall_tile && kb == 0;
-          if (!skip) {
+          if (!skip && leader) {
+            armed |= 1u << stage;
+            armed_par = (armed_par & ~(1u << stage)) | (static_cast<uint32_t>(phase) << stage);
+          }
+          if (!skip && issuer) {
             uint8_t* a_dst = tiles + stage * L::kStageBytes;
             uint8_t* b_dst = a_dst + L::kABytes;
-            if (leader) {
-              mbar_arrive_expect_tx(&full_bar[stage], 2 * L::kTxBytes);
-              armed |= 1u << stage;
-              armed_par = (armed_par & ~(1u << stage)) | (static_cast<uint32_t>(phase) << stage);
-            }
+            if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * L::kTxBytes);
             const uint32_t fb = mapa_shared(&full_bar[stage], 0);
             tma_load_2d_pair(a_dst, &tmA, fb, kb * kStageK, a_row);
             if (BMN) {  // this CTA's BN/2 output columns as 64-column boxes
@@ -248,14 +256,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         if (!ok) break;
       }
-      retire_claims(p.ws);
+      if (issuer) retire_claims(p.ws);
       // the leader's barriers count both CTAs' bytes; the final cluster barrier keeps the peer
       // resident until this drain is over
       if (leader && guard->abort) drain_armed_stages<S>(full_bar, armed, armed_par, guard->limit);
     }
   } else if (warp == 1) {
     // -------------------------------------------------------------- MMA issuer (leader only)
-    if (leader && lane == 0) {
+    if (leader) {
+      const bool issuer = elect_one();
       constexpr uint32_t idesc = OP == kOpI8 ? idesc_i8(kTileM, BN)
                                              : idesc_f16(kTileM, BN, OP == kOp16 && BF16, BMN);
       static_assert(!BMN || (BN / 2) % 64 == 0, "MN-major B halves are whole 64-column boxes");
@@ -264,27 +273,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int tiles_done = 0;    // overlapped accumulators: tiles issued so far
       const uint32_t tiles_addr = smem_u32(tiles);
       while (true) {
-        if (!mbar_wait_cluster(&schf_bar[q], qphase, guard, err, kDevTimeoutMma)) break;
+        if (!mbar_wait_cluster_warp(&schf_bar[q], qphase, guard, err, kDevTimeoutMma)) break;
         const bool valid = ring[q].rows > 0;
         const int n0 = ring[q].n0;
-        mbar_arrive(&sche_bar[q]);
+        __syncwarp();
+        if (issuer) mbar_arrive(&sche_bar[q]);
         if (++q == kSchedDepth) { q = 0; qphase ^= 1; }
         if (!valid) break;
         if (kOverlap) {
           // the previous tile's overlapped columns are read (and, the epilogue being in tile
           // order, every column of the tile before it); acce_bar[0] completes once per tile
-          if (tiles_done > 0 && !mbar_wait_cluster(&acce_bar[0], (tiles_done - 1) & 1, guard, err,
-                                                   kDevTimeoutMma))
+          if (tiles_done > 0 && !mbar_wait_cluster_warp(&acce_bar[0], (tiles_done - 1) & 1, guard,
+                                                        err, kDevTimeoutMma))
             break;
           ++tiles_done;
-        } else if (!mbar_wait_cluster(&acce_bar[acc], aphase ^ 1, guard, err, kDevTimeoutMma)) {
+        } else if (!mbar_wait_cluster_warp(&acce_bar[acc], aphase ^ 1, guard, err, kDevTimeoutMma)) {
           break;
         }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * kAccStride;
         bool ok = true;
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait_cluster(&full_bar[stage], phase, guard, err, kDevTimeoutMma)) {
+          if (!mbar_wait_cluster_warp(&full_bar[stage], phase, guard, err, kDevTimeoutMma)) {
             ok = false;
             break;
           }
@@ -294,48 +304,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const uint64_t bdesc = BMN ? sdesc_sw128_mnmajor(a_addr + L::kABytes, 8192)
                                      : sdesc_sw128_kmajor(a_addr + L::kABytes);
           constexpr uint64_t kBStep = BMN ? (2048 >> 4) : 2;
-          if constexpr (MX) {
-            // scales of this stage into TMEM (in order with the MMAs below and the previous
-            // stage's): A's 128 rows, then B's rows as kSfbAtoms 4-column atoms
-            const uint32_t sf_addr = a_addr + L::kABytes + L::kBBytes;
-            const uint32_t kSfaCol = kOverlap ? 448u + 16u * sf_slot
-                                     : sf_slot < kSfSlotsPerGap
-                                         ? BN + 16u * sf_slot
-                                         : 256u + BN + 16u * (sf_slot - kSfSlotsPerGap);
-            const uint32_t kSfbCol = kSfaCol + 4;
-            if (++sf_slot == kSfSlots) sf_slot = 0;
-            tmem_cp_32x128b_x4_pair(tmem_base + kSfaCol, sdesc_rows16(sf_addr));
+          if (issuer) {
+            if constexpr (MX) {
+              // scales of this stage into TMEM (in order with the MMAs below and the previous
+              // stage's): A's 128 rows, then B's rows as kSfbAtoms 4-column atoms
+              const uint32_t sf_addr = a_addr + L::kABytes + L::kBBytes;
+              const uint32_t kSfaCol = kOverlap ? 448u + 16u * sf_slot
+                                       : sf_slot < kSfSlotsPerGap
+                                           ? BN + 16u * sf_slot
+                                           : 256u + BN + 16u * (sf_slot - kSfSlotsPerGap);
+              const uint32_t kSfbCol = kSfaCol + 4;
+              tmem_cp_32x128b_x4_pair(tmem_base + kSfaCol, sdesc_rows16(sf_addr));
 #pragma unroll
-            for (int i = 0; i < L::kSfbAtoms; ++i)
-              tmem_cp_32x128b_x4_pair(tmem_base + kSfbCol + 4 * i,
-                                      sdesc_rows16(sf_addr + 512 * (i + 1)));
-            // weight row w of the tile has its scales in column (first row % 128 + w) / 32
-            const uint32_t sfb_col =
-                kSfbCol + static_cast<uint32_t>(((epi_glu(EPI) ? 2 * n0 : n0) & 127) >> 5);
-            constexpr uint32_t kIdesc = idesc_mxf8(kTileM, BN);
+              for (int i = 0; i < L::kSfbAtoms; ++i)
+                tmem_cp_32x128b_x4_pair(tmem_base + kSfbCol + 4 * i,
+                                        sdesc_rows16(sf_addr + 512 * (i + 1)));
+              // weight row w of the tile has its scales in column (first row % 128 + w) / 32
+              const uint32_t sfb_col =
+                  kSfbCol + static_cast<uint32_t>(((epi_glu(EPI) ? 2 * n0 : n0) & 127) >> 5);
+              constexpr uint32_t kIdesc = idesc_mxf8(kTileM, BN);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)  // K step kk uses scale byte kk of each TMEM word
-              mma_mxf8_ss_pair(d_tmem, adesc + 2 * kk, bdesc + 2 * kk,
-                               idesc_sf_ids(kIdesc, kk, kk),
-                               (tmem_base + kSfaCol) | (static_cast<uint32_t>(kk) << 30),
-                               (tmem_base + sfb_col) | (static_cast<uint32_t>(kk) << 30),
-                               (kb | kk) != 0);
-          } else {
+              for (int kk = 0; kk < 4; ++kk)  // K step kk uses scale byte kk of each TMEM word
+                mma_mxf8_ss_pair(d_tmem, adesc + 2 * kk, bdesc + 2 * kk,
+                                 idesc_sf_ids(kIdesc, kk, kk),
+                                 (tmem_base + kSfaCol) | (static_cast<uint32_t>(kk) << 30),
+                                 (tmem_base + sfb_col) | (static_cast<uint32_t>(kk) << 30),
+                                 (kb | kk) != 0);
+            } else {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {  // four 32-byte K steps per 128-byte stage row
-            if (OP == kOpI8)
-              mma_i8_ss_pair(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
-            else if (OP == kOpE4M3)
-              mma_f8_ss_pair(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
-            else
-              mma_f16_ss_pair(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
+              for (int kk = 0; kk < 4; ++kk) {  // four 32-byte K steps per 128-byte stage row
+                const uint64_t ad = adesc + 2 * kk, bd = bdesc + kBStep * kk;
+                if (OP == kOpI8)
+                  mma_i8_ss_pair(d_tmem, ad, bd, idesc, (kb | kk) != 0);
+                else if (OP == kOpE4M3)
+                  mma_f8_ss_pair(d_tmem, ad, bd, idesc, (kb | kk) != 0);
+                else
+                  mma_f16_ss_pair(d_tmem, ad, bd, idesc, (kb | kk) != 0);
+              }
+            }
+            mma_commit_pair(&empty_bar[stage], 0x3);
           }
-          }
-          mma_commit_pair(&empty_bar[stage], 0x3);
+          if (MX && ++sf_slot == kSfSlots) sf_slot = 0;
+          __syncwarp();
           if (++stage == S) { stage = 0; phase ^= 1; }
         }
         if (!ok) break;
-        mma_commit_pair(&accf_bar[acc], 0x3);
+        if (issuer) mma_commit_pair(&accf_bar[acc], 0x3);
         if (++acc == 2) { acc = 0; aphase ^= 1; }
       }
     }

@@ -80,6 +80,26 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, WaitGu
   }
 }
 
+// One lane of a converged warp, the same in every call of this kernel's warp. A warp that runs its
+// loop whole and issues through the elected lane keeps addresses and descriptors warp-uniform, which a
+// lone thread (`if (lane == 0)`) does not: a 128-byte K step of four MMAs took lone threads 270 ns,
+// whatever the size of the MMAs, and takes elected ones 197 (two loads, N = 16).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
+}
+
+// mbar_wait by all lanes of a warp; false if it failed in any of them.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, WaitGuard* g,
+                                               int* err, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, g, err, code));
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* tm) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tm)) : "memory");
@@ -324,6 +344,11 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
       return false;
     }
   }
+}
+
+__device__ __forceinline__ bool mbar_wait_cluster_warp(uint64_t* bar, uint32_t parity,
+                                                       WaitGuard* g, int* err, int code) {
+  return __all_sync(0xffffffffu, mbar_wait_cluster(bar, parity, g, err, code));
 }
 
 // 2D tiled load into this CTA's shared memory whose completion is counted on the mbarrier at
