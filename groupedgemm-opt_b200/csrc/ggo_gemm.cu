@@ -443,8 +443,8 @@ int gemm_common(const void* input, const void* weights, void* output, const int6
   const bool bf16 = dtype == GGO_DTYPE_BF16;
   int bn = choose_bn(tile_config, rows, swiglu ? 2 * n : n, num_segments, g_sm_count[dev]);
   // int8: few rows over several experts are as many row blocks as experts, not rows / 128, and wide
-  // skinny tiles keep more weight bytes in flight. 16 rows over 8 experts, N = 14336, K = 4096: 91 us
-  // with 256-wide tiles, 107 us with 128; 16 rows of one expert, N = K = 4096: 25 and 19 us.
+  // skinny tiles keep more weight bytes in flight. 16 rows over 8 experts, N = 14336, K = 4096: 78 us
+  // with 256-wide tiles, 83 us with 128; 16 rows of one expert, N = K = 4096: 17 and 13 us.
   if (i8 && bn == 128 && tile_config == GGO_TILE_AUTO) {
     const int64_t blocks = rows < num_segments ? rows : num_segments;
     if (blocks * ((n + 255) / 256) >= g_sm_count[dev]) bn = 256;

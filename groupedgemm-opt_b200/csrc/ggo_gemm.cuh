@@ -125,8 +125,9 @@ struct TileInfo {
 };
 
 // THIN: a launch of at most kSkinnyRows rows, whose tiles are all skinny: the A slot holds the skinny
-// box only, nothing is staged for TMA stores, and the room goes to more stages: 128 or 160 KB of weights
-// in flight instead of 96 or 128.
+// box only, nothing is staged for TMA stores, and the room goes to more stages: 128 or 160 KB of
+// weights in flight instead of 96 or 128. 16 rows over 8 experts: N = 14336, K = 4096 85 -> 82 us,
+// N = 4096, K = 14336 81 -> 76 us, gate/up of F = 14336 149 -> 142 us.
 template <int BN, bool THIN = false>
 struct SmemLayout {
   static constexpr int kStages = THIN ? (BN == 256 ? 5 : 8) : (BN == 256 ? 4 : 6);
@@ -577,8 +578,8 @@ __device__ __forceinline__ void store_tile_rows(uint32_t t_row, int n0, int n_ou
         load_out32<BN, EPI, BF16, I8>(t_row, nx, *reinterpret_cast<uint32_t(*)[16]>(o), rs,
                                   cs_row ? cs_row + n0 + nx : nullptr, n_out - (n0 + nx),
                                   cs_up_off);
-        load_out32<BN, EPI, BF16, I8>(t_row, nx + 32, *reinterpret_cast<uint32_t(*)[16]>(o + 16), rs,
-                                  cs_row ? cs_row + n0 + nx + 32 : nullptr,
+        load_out32<BN, EPI, BF16, I8>(t_row, nx + 32, *reinterpret_cast<uint32_t(*)[16]>(o + 16),
+                                  rs, cs_row ? cs_row + n0 + nx + 32 : nullptr,
                                   n_out - (n0 + nx + 32), cs_up_off);
       }
     }
@@ -985,9 +986,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       // column scales: one per weight row, [E, n_b] (gate rows then up rows for SwiGLU)
       const float* cs_row =
           kScaled ? p.col_scale + static_cast<size_t>(info.seg % p.num_experts) * p.n_b : nullptr;
-      store_tile_rows<BN, EPI, BF16, OutT, OP == kOpI8>(t_row, info.n0, p.n_out, row_ok, out_row, warp_tma, &tmC,
-                                     staging + ew * 4096, info.row0 + ew * 32, rs, cs_row,
-                                     p.n_b / 2, p.origin != nullptr);
+      store_tile_rows<BN, EPI, BF16, OutT, OP == kOpI8>(
+          t_row, info.n0, p.n_out, row_ok, out_row, warp_tma, &tmC, staging + ew * 4096,
+          info.row0 + ew * 32, rs, cs_row, p.n_b / 2, p.origin != nullptr);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&acce_bar[acc]);

@@ -381,11 +381,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // overlapped accumulators: the columns shared with the other accumulator first (the last
       // 64 of accumulator 0, the first 64 of accumulator 1), then release the next tile's MMAs
       constexpr int kBoxes = kOutBN / 64;
-      store_tile_rows<BN, EPI, BF16, OutT, OP == kOpI8>(t_row, info.n0, p.n_out, row_ok, out_row, warp_tma, &tmC,
-                                     staging + ew * 4096, info.row0 + wrow0, rs, cs_row,
-                                     p.n_b / 2, p.origin != nullptr,
-                                     kOverlap ? (acc == 0 ? kBoxes - 1 : 0) : 0,
-                                     kOverlap ? mapa_shared(&acce_bar[0], 0) : 0u);
+      store_tile_rows<BN, EPI, BF16, OutT, OP == kOpI8>(
+          t_row, info.n0, p.n_out, row_ok, out_row, warp_tma, &tmC, staging + ew * 4096,
+          info.row0 + wrow0, rs, cs_row, p.n_b / 2, p.origin != nullptr,
+          kOverlap ? (acc == 0 ? kBoxes - 1 : 0) : 0,
+          kOverlap ? mapa_shared(&acce_bar[0], 0) : 0u);
       tc_fence_before();
       __syncwarp();
       if (!kOverlap && lane == 0) mbar_arrive_cluster(mapa_shared(&acce_bar[acc], 0));

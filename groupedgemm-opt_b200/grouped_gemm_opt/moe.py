@@ -116,7 +116,8 @@ def moe_router(router_logits: torch.Tensor, top_k: int,
         balance_loss = E * sum_e f_e * p_e          # 1 when balanced
 
     The loss's gradient reaches the logits through p, that of ``topk_weights`` through the chosen
-    logits; one kernel computes both.
+    logits; one kernel computes both. The loss is over the tokens of this call (with expert
+    parallelism: this rank's).
 
     Args:
         router_logits: [T, E] fp32, bf16 or fp16 on the GPU, E <= 1024.

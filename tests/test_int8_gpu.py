@@ -479,3 +479,24 @@ def test_products_on_two_streams_at_once():
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
     check_device_errors(0)
+
+
+@pytest.mark.parametrize("experts,rows", [(256, 40), (257, 64), (300, 63), (1024, 50), (1000, 2500)])
+def test_many_experts(experts, rows):
+    """Both ways of ordering the segments, in thin and ordinary launches; most experts have no rows."""
+    from grouped_gemm_opt import check_device_errors, grouped_gemm_opt, grouped_gemm_opt_int8
+    g = torch.Generator().manual_seed(experts)
+    which = torch.randint(0, experts, (rows,), generator=g)
+    which[: rows // 4] = experts - 1
+    counts = torch.bincount(which, minlength=experts).tolist()
+    x, xs, w, ws = operands(counts, 48, 64, seed=1)
+    ref = reference(counts, x, xs, w, ws)
+    dev = [t.to(DEV) for t in (x, xs, w, ws, torch.tensor(counts))]
+    for sort in (True, False):
+        out = grouped_gemm_opt_int8(*dev, sort_by_m=sort)
+        assert_product(out, ref, torch.bfloat16)
+    # the bf16 product of the same codes (whole numbers up to 127 are exact in bf16)
+    plain = grouped_gemm_opt(dev[0].to(torch.bfloat16), dev[2].to(torch.bfloat16), dev[4])
+    one = [torch.ones_like(dev[1]), torch.ones_like(dev[3])]
+    assert torch.equal(plain, grouped_gemm_opt_int8(dev[0], one[0], dev[2], one[1], dev[4]))
+    check_device_errors(0)
