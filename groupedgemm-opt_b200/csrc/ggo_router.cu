@@ -184,27 +184,22 @@ __device__ __forceinline__ int choose_top_k(uint32_t (&k)[V], const TL* __restri
   return id;
 }
 
-// One warp per token. grid = ceil(T / kTokens), NW warps: 8, or 32 (a token each) when the blocks
-// would not fill the GPU. Bound by issue slots (70 % of them used, 580 instructions a token of 256
-// experts): 32768 x 256 in bf16 25 us, of which reading takes 3. table[b][e] receives block b's choices of expert e, all in the low and
-// kept in the high 16 bits; psum[b][e] the block's sum of P over kept tokens; row_stat[t] =
-// (max logit, 1 / sum exp(l - max)), the second 0 for tokens that are not kept.
+// What one block makes of its tokens, a warp each at a time (NW warps; tokens t0 + warp, + NW, ...):
+// ids, weights and row_stat[t] = (max logit, 1 / sum exp(l - max)), the second 0 for tokens that are
+// not kept; in shared memory hist[e], the block's choices of expert e, all in the low and kept in the
+// high 16 bits, and wsum[warp][e], the warps' sums of P over kept tokens. Ends with a barrier.
 template <typename TL, int V, bool VEC, int NW>
-__global__ void __launch_bounds__(32 * NW)
-    router_kernel(const TL* __restrict__ logits, const uint8_t* __restrict__ mask, int T, int E,
-                  int K, int32_t* __restrict__ ids, float* __restrict__ weights,
-                  float2* __restrict__ row_stat, uint32_t* __restrict__ table,
-                  float* __restrict__ psum) {
-  extern __shared__ uint32_t sm[];
-  uint32_t* hist = sm;                                    // [E]
-  float* wsum = reinterpret_cast<float*>(sm + E);         // [NW][E]
+__device__ __forceinline__ void route_block(const TL* __restrict__ logits,
+                                            const uint8_t* __restrict__ mask, int T, int E, int K,
+                                            int32_t* __restrict__ ids, float* __restrict__ weights,
+                                            float2* __restrict__ row_stat, int t0, uint32_t* hist,
+                                            float* wsum) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e < E; e += 32 * NW) hist[e] = 0;
   __syncthreads();
   float acc[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
-  const int t0 = blockIdx.x * kTokens;
   for (int t = t0 + warp; t < min(T, t0 + kTokens); t += NW) {
     const TL* row = logits + static_cast<size_t>(t) * E;
     alignas(16) TL x[V];
@@ -252,6 +247,23 @@ __global__ void __launch_bounds__(32 * NW)
     if (VEC || e < E) wsum[warp * E + e] = acc[i];
   }
   __syncthreads();
+}
+
+// The first of two launches. grid = ceil(T / kTokens), NW warps: 8, or 32 (a token each) when the blocks
+// would not fill the GPU. table[b][e] and psum[b][e] receive block b's hist and its sum of P. Bound by
+// issue slots (70 % of them used, 580 instructions a token of 256 experts): 32768 x 256 in bf16 25 us,
+// of which reading takes 3.
+template <typename TL, int V, bool VEC, int NW>
+__global__ void __launch_bounds__(32 * NW)
+    router_kernel(const TL* __restrict__ logits, const uint8_t* __restrict__ mask, int T, int E,
+                  int K, int32_t* __restrict__ ids, float* __restrict__ weights,
+                  float2* __restrict__ row_stat, uint32_t* __restrict__ table,
+                  float* __restrict__ psum) {
+  extern __shared__ uint32_t sm[];
+  uint32_t* hist = sm;                                    // [E]
+  float* wsum = reinterpret_cast<float*>(sm + E);         // [NW][E]
+  route_block<TL, V, VEC, NW>(logits, mask, T, E, K, ids, weights, row_stat, blockIdx.x * kTokens,
+                              hist, wsum);
   for (int e = threadIdx.x; e < E; e += 32 * NW) {
     float p = 0.f;
 #pragma unroll
@@ -264,6 +276,122 @@ __global__ void __launch_bounds__(32 * NW)
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");
+}
+
+// Over the experts, thread e of 1024 giving expert e's choices, kept choices and sum of P (threads
+// behind E zeros): the exclusive sum of the choices, and of all the kept choices and n_e sum P. Within
+// warps, then over the warps' sums: the order is fixed. Contains a barrier.
+struct ExpertScan {
+  int start;
+  long long choices;  // top_k T'
+  double sum_np;      // sum_e n_e sum_t P
+};
+
+__device__ __forceinline__ ExpertScan scan_experts(int mine, int mine_kept, double p, int E) {
+  __shared__ int warp_tot[32], warp_kept[32];
+  __shared__ double warp_term[32];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  double term = static_cast<double>(mine_kept) * p;
+  int scan = mine, ksum = mine_kept;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(kAll, scan, o);
+    if (lane >= o) scan += v;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    ksum += __shfl_xor_sync(kAll, ksum, o);
+    term += __shfl_xor_sync(kAll, term, o);
+  }
+  if (lane == 31) {
+    warp_tot[wid] = scan;
+    warp_kept[wid] = ksum;
+    warp_term[wid] = term;
+  }
+  __syncthreads();
+  ExpertScan r{scan - mine, 0, 0.0};
+  for (int w = 0; w < (E + 31) / 32; ++w) {
+    if (w < wid) r.start += warp_tot[w];
+    r.choices += warp_kept[w];
+    r.sum_np += warp_term[w];
+  }
+  return r;
+}
+
+// loss = E sum_e (n_e / choices) (sum_t P / T'), coef_e = E (n_e / choices) / T', T' = choices / K.
+__device__ __forceinline__ void write_totals(const ExpertScan& sc, int mine, int mine_kept, int E,
+                                             int K, int64_t* __restrict__ tpe,
+                                             int64_t* __restrict__ kept_counts,
+                                             float* __restrict__ loss, float* __restrict__ coef) {
+  const int tid = threadIdx.x;
+  const double n = static_cast<double>(sc.choices);
+  const double scale = sc.choices > 0 ? static_cast<double>(E) * K / (n * n) : 0.0;
+  if (tid < E) {
+    tpe[tid] = mine;
+    kept_counts[tid] = mine_kept;
+    coef[tid] = static_cast<float>(scale * mine_kept);
+  }
+  if (tid == 0) *loss = static_cast<float>(scale * sc.sum_np);
+}
+
+// The whole forward in one launch, for up to 8 x 32 tokens and 256 experts: one cluster, a block of 32
+// warps per 32 tokens, a token each. The blocks hand one another their counts and sums through
+// distributed shared memory and each writes its row of the offset table. 256 x 256 in fp32: 10.6 us, two
+// launches 12.6.
+constexpr int kSmallBlocks = 8;
+template <typename TL, int V, bool VEC>
+__global__ void __launch_bounds__(1024)
+    router_small_kernel(const TL* __restrict__ logits, const uint8_t* __restrict__ mask, int T,
+                        int E, int K, int32_t* __restrict__ ids, float* __restrict__ weights,
+                        float2* __restrict__ row_stat, int* __restrict__ table,
+                        int64_t* __restrict__ tpe, int64_t* __restrict__ kept_counts,
+                        float* __restrict__ loss, float* __restrict__ coef) {
+  extern __shared__ uint32_t sm[];
+  uint32_t* hist = sm;                             // [E]
+  float* wsum = reinterpret_cast<float*>(sm + E);  // [32][E], then [2][kSmallBlocks][E]
+  const int tid = threadIdx.x;
+  unsigned rank, nblocks;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(nblocks));
+  route_block<TL, V, VEC, 32>(logits, mask, T, E, K, ids, weights, row_stat, rank * kTokens, hist,
+                              wsum);
+  float p = 0.f;
+  if (tid < E) {
+#pragma unroll
+    for (int w = 0; w < 32; ++w) p += wsum[w * E + tid];
+  }
+  cluster_barrier();  // every block has read its wsum: the room is now the mailboxes
+  if (tid < E) {
+    const uint32_t box = static_cast<uint32_t>(
+        __cvta_generic_to_shared(wsum + rank * static_cast<unsigned>(E) + tid));
+    for (unsigned r = 0; r < nblocks; ++r) {
+      uint32_t to;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(box), "r"(r));
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(hist[tid]) : "memory");
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + kSmallBlocks * E * 4), "f"(p)
+                   : "memory");
+    }
+  }
+  cluster_barrier();
+  const uint32_t* counts = reinterpret_cast<const uint32_t*>(wsum);
+  const float* sums = wsum + kSmallBlocks * E;
+  int all = 0, kept = 0, before = 0;
+  double ps = 0.0;
+  if (tid < E) {
+    for (unsigned r = 0; r < nblocks; ++r) {
+      const uint32_t v = counts[r * E + tid];
+      if (r < rank) before += v & 0xffffu;
+      all += v & 0xffffu;
+      kept += v >> 16;
+      ps += sums[r * E + tid];
+    }
+  }
+  const ExpertScan sc = scan_experts(all, kept, ps, E);
+  if (tid < E) {
+    table[rank * E + tid] = sc.start + before;
+    if (rank == 0) table[nblocks * E + tid] = sc.start;
+  }
+  if (rank == 0) write_totals(sc, all, kept, E, K, tpe, kept_counts, loss, coef);
 }
 
 // One cluster of up to 8 CTAs x 1024 threads; CTA r owns experts [r * CE, (r+1) * CE). Thread
@@ -284,8 +412,6 @@ __global__ void __launch_bounds__(1024)
   __shared__ int tot_kept[kMaxE];
   __shared__ double tot_p[kMaxE];
   __shared__ int start[kMaxE];
-  __shared__ int warp_tot[32], warp_kept[32];
-  __shared__ double warp_term[32];
   unsigned rank, ncta;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ncta));
@@ -337,38 +463,10 @@ __global__ void __launch_bounds__(1024)
     }
   }
   cluster_barrier();
-  // exclusive scan of the totals over experts, the sum of kept choices and the loss (every CTA
-  // alike): within warps, then over the warps' sums
-  const int lane = tid & 31, wid = tid >> 5;
   const int mine = tid < E ? tot[tid] : 0;
   const int mine_kept = tid < E ? tot_kept[tid] : 0;
-  double term = tid < E ? static_cast<double>(mine_kept) * tot_p[tid] : 0.0;
-  int scan = mine, ksum = mine_kept;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(kAll, scan, o);
-    if (lane >= o) scan += v;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    ksum += __shfl_xor_sync(kAll, ksum, o);
-    term += __shfl_xor_sync(kAll, term, o);
-  }
-  if (lane == 31) {
-    warp_tot[wid] = scan;
-    warp_kept[wid] = ksum;
-    warp_term[wid] = term;
-  }
-  __syncthreads();
-  int before = 0;
-  long long choices = 0;  // top_k T'
-  double sum_np = 0.0;    // sum_e n_e sum_t P
-  for (int w = 0; w < (E + 31) / 32; ++w) {
-    if (w < wid) before += warp_tot[w];
-    choices += warp_kept[w];
-    sum_np += warp_term[w];
-  }
-  start[tid] = before + scan - mine;
+  const ExpertScan sc = scan_experts(mine, mine_kept, tid < E ? tot_p[tid] : 0.0, E);
+  start[tid] = sc.start;
   __syncthreads();
   if (active) {
     const int first = start[e];
@@ -382,17 +480,7 @@ __global__ void __launch_bounds__(1024)
       run += v;
     }
   }
-  if (rank == 0) {
-    // loss = E sum_e (n_e / choices) (sum_t P / T'), coef_e = E (n_e / choices) / T'
-    const double scale =
-        choices > 0 ? static_cast<double>(E) * K / (static_cast<double>(choices) * choices) : 0.0;
-    if (tid < E) {
-      tpe[tid] = mine;
-      kept_counts[tid] = mine_kept;
-      coef[tid] = static_cast<float>(scale * mine_kept);
-    }
-    if (tid == 0) *loss = static_cast<float>(scale * sum_np);
-  }
+  if (rank == 0) write_totals(sc, mine, mine_kept, E, K, tpe, kept_counts, loss, coef);
 }
 
 // One warp per token, persistent over tokens so that a lane's coefficients stay in registers. Every
@@ -522,6 +610,45 @@ int launch_router(const void* logits, const uint8_t* mask, int T, int E, int K, 
 }
 
 template <typename TL, int V, bool VEC>
+int launch_small_as(const void* logits, const uint8_t* mask, int T, int E, int K, int32_t* ids,
+                    float* w, float2* stat, int* table, int64_t* tpe, int64_t* kept, float* loss,
+                    float* coef, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks_for(T), 1, 1);
+  cfg.blockDim = dim3(1024, 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(E) * 33 * 4;  // at most 33 KB
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks_for(T);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, router_small_kernel<TL, V, VEC>,
+                                         static_cast<const TL*>(logits), mask, T, E, K, ids, w,
+                                         stat, table, tpe, kept, loss, coef))
+    return cuda_fail(static_cast<int>(e));
+  return check_launch();
+}
+
+template <typename TL, int V>
+int launch_small(const void* logits, const uint8_t* mask, int T, int E, int K, int32_t* ids,
+                 float* w, float2* stat, int* table, int64_t* tpe, int64_t* kept, float* loss,
+                 float* coef, cudaStream_t stream) {
+  if constexpr (V > 8) {
+    return GGO_ERR_SHAPE;
+  } else {
+    if constexpr (V * sizeof(TL) >= 4)
+      if (vec_rows<TL, V>(logits, nullptr, E))
+        return launch_small_as<TL, V, true>(logits, mask, T, E, K, ids, w, stat, table, tpe, kept,
+                                            loss, coef, stream);
+    return launch_small_as<TL, V, false>(logits, mask, T, E, K, ids, w, stat, table, tpe, kept,
+                                         loss, coef, stream);
+  }
+}
+
+template <typename TL, int V, bool VEC>
 int launch_backward_as(const void* logits, const float2* stat, const int32_t* ids, const float* w,
                        const float* coef, const float* gw, const float* gl, int T, int E, int K,
                        void* out, cudaStream_t stream) {
@@ -599,6 +726,12 @@ int ggo_moe_router(const void* logits_dev, int dtype, int64_t num_tokens, int nu
   const int nb = ggo::blocks_for(num_tokens);
   uint32_t* table = static_cast<uint32_t*>(scratch_dev);
   float* psum = reinterpret_cast<float*>(table + (static_cast<size_t>(nb) + 1) * E);
+  if (nb > 0 && nb <= ggo::kSmallBlocks && E <= 256)
+    return GGO_ROUTER_CALL(ggo::launch_small, logits_dev, token_mask_dev, T, E, top_k,
+                           topk_ids_dev, topk_weights_dev,
+                           reinterpret_cast<float2*>(row_stat_dev),
+                           reinterpret_cast<int*>(table), tokens_per_expert_dev,
+                           balance_counts_dev, balance_loss_dev, coef_dev, stream);
   if (nb > 0) {
     const int st = GGO_ROUTER_CALL(ggo::launch_router, logits_dev, token_mask_dev, T, E, top_k,
                                    topk_ids_dev, topk_weights_dev,

@@ -356,3 +356,30 @@ def test_capture_over_a_live_eager_graph_is_refused():
     del alive
     with torch.cuda.graph(torch.cuda.CUDAGraph()):
         moe_router(leaf, 2)
+
+
+@pytest.mark.parametrize("T", [1, 31, 32, 33, 255, 256, 257])
+@pytest.mark.parametrize("E", [2, 32, 33, 255, 256, 257])
+def test_both_sides_of_the_one_launch_form(T, E):
+    """Up to 256 tokens and 256 experts the forward is one launch, beyond it two: the same routing,
+    offset table, counts and loss."""
+    from grouped_gemm_opt import _C, moe_router
+    g = torch.Generator().manual_seed(T * E)
+    l = torch.randn(T, E, generator=g)
+    mask = torch.rand(T, generator=g) < 0.8
+    k = min(E, 5)
+    ids, w, counts, kept, loss = reference(l, k, mask)
+    for rows, m in ((l, mask), (torch.cat([l, torch.full((257, E), -float("inf"))]), None)):
+        r = moe_router(rows.to(DEV), k, None if m is None else m.to(DEV))
+        assert torch.equal(r.topk_ids[:T].cpu().long(), ids)
+        assert torch.all((r.topk_weights[:T].cpu().double() - w).abs() <= P_TOL * w)
+        if m is not None:
+            assert torch.equal(r.balance_counts.cpu(), kept)
+            assert torch.equal(r.tokens_per_expert.cpu(), counts)
+            assert abs(r.balance_loss.item() - loss.item()) <= (P_TOL + 2.0 ** -20) * loss.item()
+            scratch = _C.moe_route(rows.to(DEV), k)[3]
+            assert torch.equal(r.scratch[:scratch.numel()], scratch)
+        else:  # rows without a distribution add nothing to the loss
+            want = reference(l, k)
+            assert torch.equal(r.balance_counts.cpu(), want[3])
+            assert abs(r.balance_loss.item() - want[4].item()) <= (P_TOL + 2.0 ** -20) * want[4].item()
