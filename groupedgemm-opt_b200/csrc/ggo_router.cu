@@ -318,7 +318,9 @@ __device__ __forceinline__ ExpertScan scan_experts(int mine, int mine_kept, doub
   return r;
 }
 
-// loss = E sum_e (n_e / choices) (sum_t P / T'), coef_e = E (n_e / choices) / T', T' = choices / K.
+// loss = E sum_e (n_e / choices) (sum_t P / T'), T' = choices / K. The gradient takes f only through
+// f_e - sum P f, which a constant added to f does not change: coef_e = E (f_e - 1/E) / T', so that a
+// nearly balanced router's small gradient is not the difference of two large numbers.
 __device__ __forceinline__ void write_totals(const ExpertScan& sc, int mine, int mine_kept, int E,
                                              int K, int64_t* __restrict__ tpe,
                                              int64_t* __restrict__ kept_counts,
@@ -329,7 +331,7 @@ __device__ __forceinline__ void write_totals(const ExpertScan& sc, int mine, int
   if (tid < E) {
     tpe[tid] = mine;
     kept_counts[tid] = mine_kept;
-    coef[tid] = static_cast<float>(scale * mine_kept);
+    coef[tid] = static_cast<float>(scale * (mine_kept - n / E));
   }
   if (tid == 0) *loss = static_cast<float>(scale * sc.sum_np);
 }
@@ -399,7 +401,7 @@ __global__ void __launch_bounds__(1024)
 // a warp reads 32 neighbouring experts. R is at most 32: one thread per expert adds the ranges up. Totals are exchanged through distributed shared memory.
 // 32768 x 256: 15 us, the eight SMs' share of L2 bandwidth over two passes; 256 x 256: 5 us.
 // Turns table into the dispatch's absolute start rows (in place, expert starts right behind it) and
-// writes the counts, the loss and coef[e] = E f_e / T' for the backward.
+// writes the counts, the loss and coef[e] = E (f_e - 1/E) / T' for the backward.
 __global__ void __launch_bounds__(1024)
     router_finish_kernel(uint32_t* __restrict__ table, const float* __restrict__ psum, int nblocks,
                          int E, int K, int CE, int CP, int64_t* __restrict__ tpe,

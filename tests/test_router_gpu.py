@@ -383,3 +383,31 @@ def test_both_sides_of_the_one_launch_form(T, E):
             want = reference(l, k)
             assert torch.equal(r.balance_counts.cpu(), want[3])
             assert abs(r.balance_loss.item() - want[4].item()) <= (P_TOL + 2.0 ** -20) * want[4].item()
+
+
+@pytest.mark.parametrize("T,E,k", [(64, 8, 1), (300, 12, 3), (4096, 64, 4), (1024, 512, 2)])
+def test_balanced_router_has_no_balance_gradient(T, E, k):
+    """Every expert chosen equally often: the gradient is zero, not the rounding of a difference; one
+    choice moved away leaves it as exact as the small imbalance is."""
+    from grouped_gemm_opt import moe_router
+    g = torch.Generator().manual_seed(E)
+    T = T // E * E
+    base = torch.rand(T, E, generator=g)
+    chosen = (torch.arange(T)[:, None] + torch.arange(k)[None]) % E
+    base.scatter_add_(1, chosen, 2.0 + torch.rand(T, k, generator=g))
+    leaf = base.to(DEV).requires_grad_(True)
+    r = moe_router(leaf, k)
+    assert torch.equal(r.balance_counts.cpu(), torch.full((E,), T * k // E))
+    grad, = torch.autograd.grad(r.balance_loss, leaf)
+    assert torch.count_nonzero(grad) == 0
+    base[0, chosen[0, 0]] = -3.0  # token 0 takes another expert instead
+    ref_leaf = base.clone().double().requires_grad_(True)
+    _, _, _, kept, loss = reference(ref_leaf, k)
+    want, = torch.autograd.grad(loss, ref_leaf)
+    leaf = base.to(DEV).requires_grad_(True)
+    grad, = torch.autograd.grad(moe_router(leaf, k).balance_loss, leaf)
+    p = torch.softmax(base.double(), 1)
+    off = (kept.double() / (T * k) - 1.0 / E).abs()
+    size = E / T * p * (off + (p * off).sum(1, keepdim=True))
+    assert torch.all((grad.cpu().double() - want).abs() <= 4 * (P_TOL + 12 * 2.0 ** -24) * size +
+                     2.0 ** -140)
