@@ -175,6 +175,58 @@ int launch(const void* a, const void* b, int64_t b_rows, const GemmParams& p, in
   return check_launch();
 }
 
+// CTAs per tile of a thin int8 launch (1: no split): with fewer tiles than SMs, as many (a power of two
+// up to 8) as find free SMs, while every one keeps four K steps and the mailbox holds their rows. The
+// tiles are estimated at one row block per expert that can have rows. A K step takes a CTA 0.2 us, the
+// cluster's start and the mail about 2.4 us and 0.06 a row: a split has to save more than it costs. In
+// one piece and split: 1 row, N = 512, K = 8192 18.2 and 10.5 us; 1 row, N = 4096, K = 14336 29.2 and
+// 20.7; 16 rows, N = K = 4096 13.3 and 12.8; 64 rows, N = 1024, K = 8192 22.3 and 18.4; against
+// it 60 rows, N = 4096, K = 2048 12.8 and 16.9.
+int split_parts(const GemmParams& p, int sms) {
+  const int64_t blocks = p.rows < p.num_segments ? p.rows : p.num_segments;
+  const int64_t tiles = blocks * ((p.n_out + 127) / 128);
+  const int steps = (p.k + 127) / 128;
+  int parts = 1;
+  while (2 * parts <= 8 && 2 * parts * tiles <= sms && steps / (2 * parts) >= 4 &&
+         (2 * parts - 1) * p.rows <= kMailRows)
+    parts *= 2;
+  const int64_t saved = static_cast<int64_t>(steps) * (parts - 1) * 10;  // in 0.02 us, times parts
+  return saved > static_cast<int64_t>(parts) * (120 + 3 * p.rows) ? parts : 1;
+}
+
+template <int EPI, bool BF16>
+int launch_split(const void* a, const void* b, int64_t b_rows, const GemmParams& p, int parts,
+                 int dev, cudaStream_t stream) {
+  CUtensorMap ma, mb, mc, mas;
+  memset(&mc, 0, sizeof(mc));
+  if (int st = make_map_byte(&ma, a, p.rows, p.k, kBM)) return st;
+  if (int st = make_map_byte(&mb, b, b_rows, p.k, 128)) return st;
+  if (int st = make_map_byte(&mas, a, p.rows, p.k, kSkinnyRows)) return st;
+  auto kern = grouped_gemm_kernel<128, EPI, BF16, false, kOpI8, true, true>;
+  constexpr int smem = SmemLayout<128, true, true>::kTotal;
+  int sms = 0;
+  if (int st = kernel_setup(kern, smem, dev, false, &sms)) return st;
+  GemmParams q = p;
+  q.use_tma_store = 0;
+  const int64_t blocks = p.rows < p.num_segments ? p.rows : p.num_segments;
+  const int64_t tiles = blocks * ((p.n_out + 127) / 128);
+  const int64_t clusters = tiles < sms / parts ? tiles : sms / parts;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(clusters * parts), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ma, mb, mc, mas, q)) return cuda_fail(e);
+  return check_launch();
+}
+
 // Block scales of an MX launch: base pointers and their sizes in 512-B atoms.
 struct MxScales {
   const void* a = nullptr;
@@ -349,9 +401,12 @@ int launch_scaled(const void* input, const void* weights, int64_t b_rows, GemmPa
   }
   if constexpr (OP == kOpI8) {
     if (p.rows <= kSkinnyRows && p.skinny_max == kSkinnyRows) {
-      if constexpr (!epi_glu(EPI))
+      if constexpr (!epi_glu(EPI)) {
+        const int parts = p.split_mode ? 1 : split_parts(p, g_sm_count[dev]);
+        if (parts > 1) return launch_split<EPI, BF16>(input, weights, b_rows, p, parts, dev, stream);
         if (bn == 128)
           return launch<128, EPI, BF16, false, OP, true>(input, weights, b_rows, p, dev, stream);
+      }
       return launch<256, EPI, BF16, false, OP, true>(input, weights, b_rows, p, dev, stream);
     }
   }

@@ -43,6 +43,7 @@ constexpr int kMaxSegments = 1024;
 constexpr int kSchedDepth = 4;
 constexpr int kThreads = 256;
 constexpr int kSkinnyRows = 64;   // rows of the input box a skinny tile loads (its row limit)
+constexpr int kMailRows = 192;    // split launches: rows a mailbox holds, all senders together
 
 // Operand element types of the GEMM kernels (template parameter OP).
 enum OpKind { kOp16 = 0, kOpE4M3 = 1, kOpI8 = 2 };
@@ -128,9 +129,13 @@ struct TileInfo {
 // box only, nothing is staged for TMA stores, and the room goes to more stages: 128 or 160 KB of
 // weights in flight instead of 96 or 128. 16 rows over 8 experts: N = 14336, K = 4096 85 -> 82 us,
 // N = 4096, K = 14336 81 -> 76 us, gate/up of F = 14336 149 -> 142 us.
-template <int BN, bool THIN = false>
+// SPLIT (thin, 128 weight rows): a cluster of CTAs deals a tile's K steps out among them; the others'
+// integer sums arrive in the first one's mailbox, (cluster size - 1) x rows x 128 words.
+template <int BN, bool THIN = false, bool SPLIT = false>
 struct SmemLayout {
-  static constexpr int kStages = THIN ? (BN == 256 ? 5 : 8) : (BN == 256 ? 4 : 6);
+  static_assert(!SPLIT || (THIN && BN == 128), "split launches");
+  static constexpr int kStages = SPLIT ? 4 : THIN ? (BN == 256 ? 5 : 8) : (BN == 256 ? 4 : 6);
+  static constexpr int kMailBytes = SPLIT ? kMailRows * 128 * 4 : 0;
   static constexpr int kABytes = (THIN ? kSkinnyRows : kBM) * kBK * 2;  // 8 or 16 KB
   static constexpr int kBBytes = BN * kBK * 2;    // 32 KB or 16 KB
   static constexpr int kStageBytes = kABytes + kBBytes;
@@ -139,7 +144,7 @@ struct SmemLayout {
   static constexpr int kTableBytes = 4 * kMaxSegments * 4 + 16;
   static constexpr int kMiscBytes = 1024;
   static constexpr int kTotal =
-      1024 /*align slack*/ + kTileBytes + kStagingBytes + kTableBytes + kMiscBytes;
+      1024 /*align slack*/ + kTileBytes + kStagingBytes + kTableBytes + kMiscBytes + kMailBytes;
   static_assert(kTotal <= 227 * 1024, "shared memory budget");
 };
 
@@ -688,7 +693,8 @@ struct SkinnyScales {
 template <int BN, int EPI, bool BF16, typename OutT, bool I8>
 __device__ __forceinline__ void store_skinny(uint32_t t_row, const GemmParams& p,
                                              const TileInfo& info, int ew,
-                                             const SkinnyScales<BN, EPI>& sk) {
+                                             const SkinnyScales<BN, EPI>& sk,
+                                             const uint32_t* mail = nullptr, int senders = 0) {
   constexpr bool kScaled = EPI == kEpiScaled || EPI == kEpiScaledSwiGLU;
   const int lane = threadIdx.x & 31;
   constexpr int kHalves = epi_glu(EPI) ? 1 : BN / 128;
@@ -704,6 +710,11 @@ __device__ __forceinline__ void store_skinny(uint32_t t_row, const GemmParams& p
       tmem_ld_32x32b_x8(t_row + 128 * h + cb, v);
       if (epi_glu(EPI)) tmem_ld_32x32b_x8(t_row + 128 + cb, u);
       tmem_ld_wait();
+      for (int o = 0; o < senders; ++o) {  // the other CTAs' integer sums
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (cb + j < info.rows) v[j] += mail[(o * info.rows + cb + j) * 128 + 32 * ew + lane];
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int r = cb + j;
@@ -724,13 +735,34 @@ __device__ __forceinline__ void store_skinny(uint32_t t_row, const GemmParams& p
   }
 }
 
-template <int BN, int EPI, bool BF16, bool BMN = false, int OP = kOp16, bool THIN = false>
+// A sender's part of a split tile: this warp's 32 weight rows of the accumulator into the mailbox at
+// the shared::cluster address `mail` (row j at j * 128 words).
+__device__ __forceinline__ void send_sums(uint32_t t_row, int rows, uint32_t mail, int ew) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int cb = 0; cb < rows; cb += 8) {
+    uint32_t v[8];
+    tmem_ld_32x32b_x8(t_row + cb, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (cb + j < rows)
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(
+                         mail + static_cast<uint32_t>((cb + j) * 128 + 32 * ew + lane) * 4),
+                     "r"(v[j])
+                     : "memory");
+  }
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+}
+
+template <int BN, int EPI, bool BF16, bool BMN = false, int OP = kOp16, bool THIN = false,
+          bool SPLIT = false>
 __global__ void __launch_bounds__(kThreads, 1)
     grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA,
                         const __grid_constant__ CUtensorMap tmB,
                         const __grid_constant__ CUtensorMap tmC,
                         const __grid_constant__ CUtensorMap tmAs, const GemmParams p) {
-  using L = SmemLayout<BN, THIN>;
+  using L = SmemLayout<BN, THIN, SPLIT>;
   constexpr int S = L::kStages;
   constexpr int kTmemCols = 2 * BN;             // two accumulators
   constexpr int kOutBN = epi_glu(EPI) ? BN / 2 : BN;
@@ -760,6 +792,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ring + kSchedDepth);
   int* total_tiles_s = reinterpret_cast<int*>(tmem_slot + 1);
   WaitGuard* guard = reinterpret_cast<WaitGuard*>(tmem_slot + 4);  // 16-byte aligned
+  // split launches: mail_bar[0] (first CTA) counts the senders' warps in, mail_bar[1] (senders) the
+  // first CTA's warps that have read the mailbox
+  uint64_t* mail_bar = reinterpret_cast<uint64_t*>(guard + 1);
+  uint32_t* mail = reinterpret_cast<uint32_t*>(misc + L::kMiscBytes);
+  const int parts = SPLIT ? static_cast<int>(cluster_nctarank()) : 1;
+  const int part = SPLIT ? static_cast<int>(cluster_ctarank()) : 0;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -779,6 +817,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&schf_bar[i], 1);
       mbar_init(&sche_bar[i], 1 + 4);
     }
+    if (SPLIT) {
+      mbar_init(&mail_bar[0], 4 * (parts - 1));
+      mbar_init(&mail_bar[1], 4);
+    }
     guard->abort = 0;
     guard->limit = p.wait_limit;
     fence_barrier_init();
@@ -793,6 +835,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   build_segment_table<kBM, kOutBN>(p, tiles, t_cnt, t_rowoff, t_order, t_tileoff, total_tiles_s, err);
   tc_fence_before();
   __syncthreads();
+  if (SPLIT) cluster_sync();  // barriers of the whole cluster initialised before any remote arrive
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int total_tiles = *total_tiles_s;
@@ -800,6 +843,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   // K elements per pipeline stage: one 128-B swizzle row (64 bf16/fp16 or 128 one-byte ones)
   constexpr int kStageK = OP == kOp16 ? kBK : 128;
   const int num_kb = (p.k + kStageK - 1) / kStageK;
+  const int kb_first = SPLIT ? num_kb * part / parts : 0;  // this CTA's share of a tile's K steps
+  const int kb_end = SPLIT ? num_kb * (part + 1) / parts : num_kb;
 
   if (warp == 0) {
     // -------------------------------------------------------------- TMA producer
@@ -809,10 +854,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       int stage = 0, phase = 0, q = 0, qphase = 0;
       uint32_t armed = 0, armed_par = 0;  // stages whose loads were issued, and their parity
       bool first = true;
+      int t = static_cast<int>(blockIdx.x) / parts;
       while (true) {
-        // the first tile by block index, the others by claiming
-        int t = static_cast<int>(blockIdx.x);
-        if (!first) {
+        // the first tile by block index, the others by claiming; a cluster's by turns
+        if (SPLIT) {
+          if (!first) t += static_cast<int>(gridDim.x) / parts;
+        } else if (!first) {
           if (issuer) t = static_cast<int>(gridDim.x) + atomicAdd(&p.ws->tile_counter, 1);
           t = __shfl_sync(0xffffffffu, t, issuer_lane);
         }
@@ -832,14 +879,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (++q == kSchedDepth) { q = 0; qphase ^= 1; }
         if (info.rows == 0) break;
         bool ok = true;
-        for (int kb = 0; kb < num_kb; ++kb) {
+        for (int kb = kb_first; kb < kb_end; ++kb) {
           if (!mbar_wait_warp(&empty_bar[stage], phase ^ 1, guard, err, kDevTimeoutProducer)) {
             ok = false;
             break;
           }
           // test hook: the CTA that claimed tile 0 leaves that tile's first stage unarmed, so its
           // MMA's bounded wait expires
-          const bool skip = p.inject_stall && t == 0 && kb == 0;
+          const bool skip = p.inject_stall && t == 0 && kb == kb_first;
           if (!skip && issuer) {
             uint8_t* a_dst = tiles + stage * L::kStageBytes;
             uint8_t* b_dst = a_dst + L::kABytes;
@@ -869,7 +916,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!ok) break;
       }
-      if (issuer) retire_claims(p.ws);
+      if (!SPLIT && issuer) retire_claims(p.ws);
       if (guard->abort) drain_armed_stages<S>(full_bar, armed, armed_par, guard->limit);
     }
   } else if (warp == 1) {
@@ -897,7 +944,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
         bool ok = true;
-        for (int kb = 0; kb < num_kb; ++kb) {
+        for (int kb = kb_first; kb < kb_end; ++kb) {
           if (!mbar_wait_warp(&full_bar[stage], phase, guard, err, kDevTimeoutMma)) {
             ok = false;
             break;
@@ -921,9 +968,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const uint64_t wdesc =
                       sdesc_sw128_kmajor(a_addr + L::kABytes + h * 16384) + 2 * kk;
                   if (OP == kOpI8)
-                    mma_i8_ss(d_tmem + 128 * h, wdesc, adesc + 2 * kk, idesc_s, (kb | kk) != 0);
+                    mma_i8_ss(d_tmem + 128 * h, wdesc, adesc + 2 * kk, idesc_s, ((kb - kb_first) | kk) != 0);
                   else
-                    mma_f16_ss(d_tmem + 128 * h, wdesc, adesc + 2 * kk, idesc_s, (kb | kk) != 0);
+                    mma_f16_ss(d_tmem + 128 * h, wdesc, adesc + 2 * kk, idesc_s, ((kb - kb_first) | kk) != 0);
                 }
               }
               mma_commit(&empty_bar[stage]);
@@ -932,11 +979,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {  // four 32-byte K steps per 128-byte stage row
               if (OP == kOpI8)
-                mma_i8_ss(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
+                mma_i8_ss(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, ((kb - kb_first) | kk) != 0);
               else if (OP == kOpE4M3)
-                mma_f8_ss(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
+                mma_f8_ss(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, ((kb - kb_first) | kk) != 0);
               else
-                mma_f16_ss(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, (kb | kk) != 0);
+                mma_f16_ss(d_tmem, adesc + 2 * kk, bdesc + kBStep * kk, idesc, ((kb - kb_first) | kk) != 0);
             }
             mma_commit(&empty_bar[stage]);
           }
@@ -951,7 +998,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp >= 4) {
     // -------------------------------------------------------------- epilogue
     const int ew = warp - 4;  // TMEM lane quarter this warp may access
-    int q = 0, qphase = 0, acc = 0, aphase = 0;
+    int q = 0, qphase = 0, acc = 0, aphase = 0, mphase = 0;
     while (true) {
       if (!mbar_wait(&schf_bar[q], qphase, guard, err, kDevTimeoutEpilogue)) break;
       const TileInfo info = ring[q];
@@ -974,7 +1021,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + acc * BN;
       using OutT = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
       if (THIN || (kSkinnyOk && info.skinny)) {
-        store_skinny<BN, EPI, BF16, OutT, OP == kOpI8>(t_row, p, info, ew, sk);
+        if (SPLIT && part > 0) {  // hand the sums to the cluster's first CTA
+          if (!mbar_wait_cluster_warp(&mail_bar[1], mphase ^ 1, guard, err, kDevTimeoutEpilogue))
+            break;
+          send_sums(t_row, info.rows,
+                    mapa_shared(mail + (part - 1) * info.rows * 128, 0), ew);
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa_shared(&mail_bar[0], 0));
+        } else {
+          if (SPLIT &&
+              !mbar_wait_cluster_warp(&mail_bar[0], mphase, guard, err, kDevTimeoutEpilogue))
+            break;
+          store_skinny<BN, EPI, BF16, OutT, OP == kOpI8>(t_row, p, info, ew, sk, mail, parts - 1);
+          __syncwarp();
+          if (SPLIT && lane == 0)
+            for (int o = 1; o < parts; ++o) mbar_arrive_cluster(mapa_shared(&mail_bar[1], o));
+        }
+        mphase ^= 1;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&acce_bar[acc]);
@@ -1000,6 +1063,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (p.origin) __threadfence_system();  // scattered rows visible to the peers before exit
   if (warp >= 4 && lane == 0) bulk_wait_all();  // TMA stores done before shared memory goes
   __syncthreads();
+  if (SPLIT) cluster_sync();  // no remote arrive or mail may target a CTA that has exited
   if (warp == 2) {
     tc_fence_after();
     tmem_dealloc(tmem_base, kTmemCols);

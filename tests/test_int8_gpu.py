@@ -178,6 +178,25 @@ def test_few_tiles_and_a_long_sum(counts, n, k, swiglu):
     check_device_errors(0)
 
 
+@pytest.mark.parametrize("counts", [[1], [24], [27], [28], [64], [0, 3, 0, 9], [1] * 20])
+@pytest.mark.parametrize("n,k", [(8, 16384), (136, 8192), (512, 4112), (2048, 10000), (4104, 6144)])
+def test_sums_dealt_out_to_clusters(counts, n, k):
+    """Few tiles and long sums: a cluster of two, four or eight CTAs per tile, over several tiles each,
+    in turn with launches in one piece on the same stream."""
+    from grouped_gemm_opt import check_device_errors, grouped_gemm_opt_int8
+    x, xs, w, ws = operands(counts, n, k, seed=3)
+    ref = reference(counts, x, xs, w, ws)
+    dev = [t.to(DEV) for t in (x, xs, w, ws, torch.tensor(counts))]
+    other = [t.to(DEV) for t in operands([70, 3], 64, 64)] + [torch.tensor([70, 3], device=DEV)]
+    want_other = grouped_gemm_opt_int8(*other)
+    first = grouped_gemm_opt_int8(*dev)
+    assert_product(first, ref, torch.bfloat16)
+    for _ in range(20):
+        assert torch.equal(grouped_gemm_opt_int8(*dev), first)
+        assert torch.equal(grouped_gemm_opt_int8(*other), want_other)
+    check_device_errors(0)
+
+
 def test_longest_sum_does_not_wrap():
     """K = 131056 products of -128 with -128: 2147221504, just inside 32 bits, rounded to fp32."""
     from grouped_gemm_opt import grouped_gemm_opt_int8
