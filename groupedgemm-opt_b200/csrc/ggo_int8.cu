@@ -214,7 +214,8 @@ __global__ void __launch_bounds__(256)
   extern __shared__ int psm[];
   __shared__ uint32_t s_max[8];
   int* off = psm;      // [E] running sorted position per expert
-  int* pos = psm + E;  // [kRouteTokens * K]
+  int* lim = off + E;  // [E] first sorted position behind this block's rows of the expert
+  int* pos = lim + E;  // [kRouteTokens * K] sorted position per entry, -1 for a dropped one
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t0 = blockIdx.x * kRouteTokens;
   const int ntok = min(kRouteTokens, T - t0);
@@ -233,8 +234,14 @@ __global__ void __launch_bounds__(256)
     v[2 * i] = ok ? src[2 * c] : make_uint4(0, 0, 0, 0);
     v[2 * i + 1] = ok ? src[2 * c + 1] : make_uint4(0, 0, 0, 0);
   }
-  for (int e = threadIdx.x; e < E; e += 256)
+  // the table's last row (the experts' starts) lies behind those of the blocks
+  const int* next = block_offsets + static_cast<size_t>(blockIdx.x + 1) * E;
+  const bool last = blockIdx.x + 1 == gridDim.x;
+  for (int e = threadIdx.x; e < E; e += 256) {
     off[e] = block_offsets[static_cast<size_t>(blockIdx.x) * E + e];
+    const int end = !last ? next[e] : (e + 1 < E ? next[e + 1] : T * K);
+    lim[e] = min(max(end, 0), T * K);
+  }
   __syncthreads();
   if (warp == 0) {
     const int32_t* ids = topk_ids + static_cast<size_t>(t0) * K;
@@ -243,13 +250,15 @@ __global__ void __launch_bounds__(256)
       const bool valid = i < nent;
       const unsigned vmask = __ballot_sync(kAll, valid);
       if (valid) {
-        // ids and offsets that do not belong together stay inside the buffers
-        const int id = min(max(ids[i], 0), E - 1);
+        // a choice that the table has no place for is dropped, as in the dispatch of ggo_moe.cu
+        const int id = ids[i];
+        const bool known = id >= 0 && id < E;
         const unsigned peers = __match_any_sync(vmask, id);
-        const int b = off[id];
+        const unsigned b = known ? off[id] : 0;  // unsigned: a table may hold anything
         __syncwarp(vmask);
-        if (lane == __ffs(peers) - 1) off[id] = b + __popc(peers);
-        const int ps = min(max(b + __popc(peers & ((1u << lane) - 1u)), 0), T * K - 1);
+        if (known && lane == __ffs(peers) - 1) off[id] = static_cast<int>(b + __popc(peers));
+        int ps = static_cast<int>(b + __popc(peers & ((1u << lane) - 1u)));
+        if (!known || ps < 0 || ps >= lim[id]) ps = -1;
         pos[i] = ps;
         if (blockIdx.y == 0) slot_pos[static_cast<size_t>(t0) * K + i] = ps;
       }
@@ -272,12 +281,15 @@ __global__ void __launch_bounds__(256)
     for (int w = 0; w < WPT; ++w) m = __vmaxu2(m, s_max[first + w]);
   }
   const RowCode rc = row_code<T16>(m);
-  if (at < K) scale_sorted[pos[tl * K + at]] = rc.scale;
+  if (at < K && pos[tl * K + at] >= 0) scale_sorted[pos[tl * K + at]] = rc.scale;
   auto put = [&](int c, const uint4& a, const uint4& b) {
     const uint2 lo = code8<T16>(a, rc), hi = code8<T16>(b, rc);
-    for (int j = 0; j < K; ++j)
-      reinterpret_cast<uint4*>(q_sorted + static_cast<size_t>(pos[tl * K + j]) * H)[c] =
-          make_uint4(lo.x, lo.y, hi.x, hi.y);
+    for (int j = 0; j < K; ++j) {
+      const int ps = pos[tl * K + j];
+      if (ps >= 0)
+        reinterpret_cast<uint4*>(q_sorted + static_cast<size_t>(ps) * H)[c] =
+            make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
   };
 #pragma unroll
   for (int i = 0; i < P; ++i)
@@ -324,7 +336,7 @@ int launch_permute(const void* x, int T, int H, int E, int K, const int32_t* ids
                    const int* offsets, uint8_t* q, float* scale, int32_t* slot_pos,
                    cudaStream_t stream) {
   const int nb = (T + kRouteTokens - 1) / kRouteTokens;
-  const size_t smem = (static_cast<size_t>(E) + kRouteTokens * K) * 4;  // at most 6 KB
+  const size_t smem = (2 * static_cast<size_t>(E) + kRouteTokens * K) * 4;  // at most 10 KB
   const T16* xp = static_cast<const T16*>(x);
   // Few tokens: all eight warps on one, so that every SM has a row. Else as many as hold a row of that
   // length in their registers. 16384 tokens x 4096 columns, two choices: 48 us (5.6 TB/s); 67 us with

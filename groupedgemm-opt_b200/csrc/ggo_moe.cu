@@ -166,6 +166,7 @@ struct DispatchTargets {
   int world;
   int rank;
   int el;
+  int capacity;  // rows of every receive buffer
   const int64_t* counts_all;
   T16* recv[kMaxPeers];
   int32_t* origin[kMaxPeers];
@@ -174,6 +175,9 @@ struct DispatchTargets {
 // grid = ceil(T / kRouteTokens). Sorted positions by one warp (deterministic in-block ranks),
 // destination rows from per-expert bases, then the row copy by all warps (each token's row read
 // once, written top_k times, four 16-byte chunks in flight per lane).
+// A choice that the offset table has no place for (an id outside [0, E), more choices of an expert
+// than this block's share, a table of another routing) is dropped with slot_pos -1, so that ids and
+// tables which do not belong together touch no other row and nothing outside the buffers.
 template <typename T16>
 __global__ void __launch_bounds__(kRouteThreads)
     dispatch_kernel(const T16* __restrict__ x, int T, int H, int E, int K,
@@ -182,17 +186,22 @@ __global__ void __launch_bounds__(kRouteThreads)
                     int32_t* __restrict__ sorted_token, int32_t* __restrict__ slot_pos) {
   extern __shared__ int psm[];
   int* off = psm;             // [E] running sorted position per expert (this block)
-  int* dbase = psm + E;       // [E] destination row of the expert's first row from this rank
-  int* pos = dbase + E;       // [kRouteTokens * K] sorted position per entry
-  int* drow = pos + kRouteTokens * K;  // [kRouteTokens * K] destination row per entry
+  int* lim = off + E;         // [E] first sorted position behind this block's rows of the expert
+  int* delta = lim + E;       // [E] destination row of the expert's rows minus their sorted position
+  int* drow = delta + E;      // [kRouteTokens * K] destination row per entry, -1 for a dropped one
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t0 = blockIdx.x * kRouteTokens;
   const int ntok = min(kRouteTokens, T - t0);
   const int nent = ntok * K;
+  const bool last = blockIdx.x + 1 == gridDim.x;
   for (int e = threadIdx.x; e < E; e += kRouteThreads) {
     off[e] = block_offsets[static_cast<size_t>(blockIdx.x) * E + e];
+    const int end = !last       ? block_offsets[static_cast<size_t>(blockIdx.x + 1) * E + e]
+                    : e + 1 < E ? expert_start[e + 1]
+                                : T * K;
+    lim[e] = min(max(end, 0), T * K);
     if (tg.world == 1) {
-      dbase[e] = expert_start[e];
+      delta[e] = 0;
     } else {
       // owner's receive buffer is expert-major: all rows of its lower local experts (from every
       // source), then this expert's rows from lower source ranks
@@ -202,7 +211,9 @@ __global__ void __launch_bounds__(kRouteThreads)
         for (int s = 0; s < tg.world; ++s)
           b += tg.counts_all[static_cast<size_t>(s) * E + r * tg.el + j];
       for (int s = 0; s < tg.rank; ++s) b += tg.counts_all[static_cast<size_t>(s) * E + e];
-      dbase[e] = static_cast<int>(b);
+      // (saturated: counts of any size move the rows out of the buffer, not round to its start)
+      b -= expert_start[e];
+      delta[e] = static_cast<int>(b < INT32_MIN ? INT32_MIN : (b > INT32_MAX ? INT32_MAX : b));
     }
   }
   __syncthreads();
@@ -214,19 +225,24 @@ __global__ void __launch_bounds__(kRouteThreads)
       const unsigned vmask = __ballot_sync(0xffffffffu, valid);
       if (valid) {
         const int id = ids[i];
+        const bool known = id >= 0 && id < E;
         const unsigned peers = __match_any_sync(vmask, id);
-        const int rank_in = __popc(peers & ((1u << lane) - 1u));
-        const int b = off[id];
+        const unsigned b = known ? off[id] : 0;  // unsigned: a table may hold anything
         __syncwarp(vmask);
-        if (lane == __ffs(peers) - 1) off[id] = b + __popc(peers);
-        const int ps = b + rank_in;
-        pos[i] = ps;
-        const int d = dbase[id] + (ps - expert_start[id]);
+        if (known && lane == __ffs(peers) - 1) off[id] = static_cast<int>(b + __popc(peers));
+        const int ps = static_cast<int>(b + __popc(peers & ((1u << lane) - 1u)));
+        int d = -1;
+        if (known && ps >= 0 && ps < lim[id]) {
+          const long long to = static_cast<long long>(ps) + delta[id];
+          if (to >= 0 && to < tg.capacity) d = static_cast<int>(to);
+        }
         drow[i] = d;
-        slot_pos[static_cast<size_t>(t0) * K + i] = ps;
-        if (sorted_token) sorted_token[ps] = t0 + i / K;
-        // origin word: source rank in bits 28..30, sorted position on the source below
-        if (tg.world > 1) tg.origin[id / tg.el][d] = (tg.rank << 28) | ps;
+        slot_pos[static_cast<size_t>(t0) * K + i] = d < 0 ? -1 : ps;
+        if (d >= 0) {
+          if (sorted_token) sorted_token[ps] = t0 + i / K;
+          // origin word: source rank in bits 28..30, sorted position on the source below
+          if (tg.world > 1) tg.origin[id / tg.el][d] = (tg.rank << 28) | ps;
+        }
       }
       __syncwarp();
     }
@@ -244,6 +260,7 @@ __global__ void __launch_bounds__(kRouteThreads)
       }
       for (int j = 0; j < K; ++j) {
         const int e = tl * K + j;
+        if (drow[e] < 0) continue;
         const int r = tg.world > 1 ? topk_ids[static_cast<size_t>(t0) * K + e] / tg.el : 0;
         uint4* dst = reinterpret_cast<uint4*>(tg.recv[r] + static_cast<size_t>(drow[e]) * H);
 #pragma unroll
@@ -275,8 +292,17 @@ __global__ void __launch_bounds__(256)
   const int lane = threadIdx.x & 31;
   if (t >= T) return;
   const int vec = H / 8;
-  if (err != nullptr && *reinterpret_cast<const volatile int*>(err) != 0) {
-    // the data this token's rows came from is incomplete: hand back NaN, never stale numbers
+  int ps[kMaxTopK];
+  float wt[kMaxTopK];
+  bool bad = err != nullptr && *reinterpret_cast<const volatile int*>(err) != 0;
+  for (int j = 0; j < K; ++j) {
+    ps[j] = slot_pos[static_cast<size_t>(t) * K + j];
+    wt[j] = w[static_cast<size_t>(t) * K + j];
+    bad |= ps[j] < 0;
+  }
+  if (bad) {
+    // this token's rows are incomplete (an expired wait, a dropped choice): hand back NaN, never
+    // stale or partial numbers
     uint4 nan4;
     T16* nh = reinterpret_cast<T16*>(&nan4);
 #pragma unroll
@@ -284,12 +310,6 @@ __global__ void __launch_bounds__(256)
     uint4* dst = reinterpret_cast<uint4*>(out + static_cast<size_t>(t) * H);
     for (int c = blockIdx.y * 32 + lane; c < vec; c += 32 * gridDim.y) dst[c] = nan4;
     return;
-  }
-  int ps[kMaxTopK];
-  float wt[kMaxTopK];
-  for (int j = 0; j < K; ++j) {
-    ps[j] = slot_pos[static_cast<size_t>(t) * K + j];
-    wt[j] = w[static_cast<size_t>(t) * K + j];
   }
   uint4* dst = reinterpret_cast<uint4*>(out + static_cast<size_t>(t) * H);
   for (int c = blockIdx.y * 32 + lane; c < vec; c += 32 * gridDim.y) {
@@ -591,26 +611,27 @@ int nblocks_for(int64_t T) { return static_cast<int>((T + kRouteTokens - 1) / kR
 template <typename T16>
 void launch_dispatch(const void* x, int T, int H, int E, int K, const int32_t* ids,
                      const int* bo, const int* es, const int64_t* counts_all, int world, int rank,
-                     void* const* recv, int32_t* const* origin, int32_t* stok, int32_t* spos,
-                     cudaStream_t stream) {
+                     int capacity, void* const* recv, int32_t* const* origin, int32_t* stok,
+                     int32_t* spos, cudaStream_t stream) {
   DispatchTargets<T16> tg;
   tg.world = world;
   tg.rank = rank;
   tg.el = E / world;
+  tg.capacity = capacity;
   tg.counts_all = counts_all;
   for (int r = 0; r < kMaxPeers; ++r) {
     tg.recv[r] = r < world ? static_cast<T16*>(recv[r]) : nullptr;
     tg.origin[r] = r < world ? origin[r] : nullptr;
   }
   const int nb = nblocks_for(T);
-  const size_t smem = (2 * static_cast<size_t>(E) + 2 * kRouteTokens * K) * 4;
+  const size_t smem = (3 * static_cast<size_t>(E) + kRouteTokens * K) * 4;  // at most 14 KB
   dispatch_kernel<T16><<<nb, kRouteThreads, smem, stream>>>(
       static_cast<const T16*>(x), T, H, E, K, ids, bo, es, tg, stok, spos);
 }
 
 int dispatch_common(const void* x, int64_t num_tokens, int64_t hidden, int E, int K,
                     const int32_t* ids, const void* scratch, const int64_t* counts_all, int world,
-                    int rank, void* const* recv, int32_t* const* origin, int32_t* stok,
+                    int rank, int64_t capacity, void* const* recv, int32_t* const* origin, int32_t* stok,
                     int32_t* spos, int dtype, cudaStream_t stream) {
   if (!x || !ids || !spos || !scratch) return GGO_ERR_INVALID_ARG;
   if (num_tokens < 0 || hidden <= 0 || E <= 0 || E > kMaxExperts || K <= 0 || K > kMaxTopK)
@@ -625,12 +646,13 @@ int dispatch_common(const void* x, int64_t num_tokens, int64_t hidden, int E, in
   if (nb == 0) return GGO_OK;
   const int* bo = static_cast<const int*>(scratch);
   const int* es = bo + static_cast<size_t>(nb) * E;
+  const int cap = static_cast<int>(capacity < INT32_MAX ? capacity : INT32_MAX);
   if (dtype == GGO_DTYPE_BF16)
     launch_dispatch<__nv_bfloat16>(x, T, static_cast<int>(hidden), E, K, ids, bo, es, counts_all,
-                                   world, rank, recv, origin, stok, spos, stream);
+                                   world, rank, cap, recv, origin, stok, spos, stream);
   else
     launch_dispatch<__half>(x, T, static_cast<int>(hidden), E, K, ids, bo, es, counts_all, world,
-                            rank, recv, origin, stok, spos, stream);
+                            rank, cap, recv, origin, stok, spos, stream);
   return ggo::check_launch();
 }
 
@@ -677,8 +699,25 @@ int ggo_moe_permute(const void* x_dev, int64_t num_tokens, int64_t hidden, int n
   void* recv[1] = {x_sorted_dev};
   int32_t* origin[1] = {nullptr};
   return ggo::dispatch_common(x_dev, num_tokens, hidden, num_experts, top_k, topk_ids_dev,
-                              scratch_dev, nullptr, 1, 0, recv, origin, sorted_token_dev,
-                              slot_pos_dev, dtype, stream);
+                              scratch_dev, nullptr, 1, 0, num_tokens * top_k, recv, origin,
+                              sorted_token_dev, slot_pos_dev, dtype, stream);
+}
+
+int ggo_ep_dispatch_bounded(const void* x_dev, int64_t num_tokens, int64_t hidden,
+                            int num_experts, int top_k, const int32_t* topk_ids_dev,
+                            const void* scratch_dev, const int64_t* counts_all_dev,
+                            int world_size, int rank, int64_t capacity_rows,
+                            void* const* recv_rows, int32_t* const* recv_origin,
+                            int32_t* slot_pos_dev, int dtype, cudaStream_t stream) {
+  if (world_size < 1 || world_size > ggo::kMaxPeers || rank < 0 || rank >= world_size ||
+      capacity_rows < 0 || !counts_all_dev || !recv_rows || !recv_origin ||
+      num_experts % world_size)
+    return GGO_ERR_INVALID_ARG;
+  for (int r = 0; r < world_size; ++r)
+    if (!recv_rows[r] || !recv_origin[r]) return GGO_ERR_INVALID_ARG;
+  return ggo::dispatch_common(x_dev, num_tokens, hidden, num_experts, top_k, topk_ids_dev,
+                              scratch_dev, counts_all_dev, world_size, rank, capacity_rows,
+                              recv_rows, recv_origin, nullptr, slot_pos_dev, dtype, stream);
 }
 
 int ggo_ep_dispatch(const void* x_dev, int64_t num_tokens, int64_t hidden, int num_experts,
@@ -686,14 +725,9 @@ int ggo_ep_dispatch(const void* x_dev, int64_t num_tokens, int64_t hidden, int n
                     const int64_t* counts_all_dev, int world_size, int rank,
                     void* const* recv_rows, int32_t* const* recv_origin, int32_t* slot_pos_dev,
                     int dtype, cudaStream_t stream) {
-  if (world_size < 1 || world_size > ggo::kMaxPeers || rank < 0 || rank >= world_size ||
-      !counts_all_dev || !recv_rows || !recv_origin || num_experts % world_size)
-    return GGO_ERR_INVALID_ARG;
-  for (int r = 0; r < world_size; ++r)
-    if (!recv_rows[r] || !recv_origin[r]) return GGO_ERR_INVALID_ARG;
-  return ggo::dispatch_common(x_dev, num_tokens, hidden, num_experts, top_k, topk_ids_dev,
-                              scratch_dev, counts_all_dev, world_size, rank, recv_rows,
-                              recv_origin, nullptr, slot_pos_dev, dtype, stream);
+  return ggo_ep_dispatch_bounded(x_dev, num_tokens, hidden, num_experts, top_k, topk_ids_dev,
+                                 scratch_dev, counts_all_dev, world_size, rank, INT32_MAX,
+                                 recv_rows, recv_origin, slot_pos_dev, dtype, stream);
 }
 
 int ggo_quantize_fp8_rows(const void* x_dev, int64_t rows, int64_t cols, int dtype, void* q_dev,

@@ -579,21 +579,29 @@ std::vector<torch::Tensor> moe_router(const torch::Tensor& logits, int64_t top_k
   return {o.begin(), o.end()};
 }
 
-// Permute with INT8 quantisation: returns (q_sorted int8 [T*k, H], scale fp32 [T*k], slot_pos int32).
-std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_permute_int8(
-    const torch::Tensor& x, const torch::Tensor& topk_ids, const torch::Tensor& scratch,
-    int64_t num_experts) {
+// What the dispatches take of a routing: ids of these tokens and the offset table of their router.
+void check_routing(const torch::Tensor& x, const torch::Tensor& topk_ids,
+                   const torch::Tensor& scratch, int64_t num_experts) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous(), "hidden must be 2D contiguous CUDA");
   TORCH_CHECK(topk_ids.scalar_type() == torch::kInt32 && topk_ids.is_contiguous() &&
                   topk_ids.dim() == 2 && topk_ids.size(0) == x.size(0) &&
                   topk_ids.device() == x.device(),
               "topk_ids must be contiguous int32 [T, top_k] on hidden's device");
-  const int64_t T = x.size(0), H = x.size(1), k = topk_ids.size(1);
   TORCH_CHECK(num_experts > 0 && num_experts <= INT32_MAX &&
-                  scratch.scalar_type() == torch::kInt32 && scratch.device() == x.device() &&
-                  static_cast<size_t>(scratch.numel()) * 4 >=
-                      ggo_moe_route_scratch_bytes(T, static_cast<int>(num_experts)),
+                  scratch.scalar_type() == torch::kInt32 && scratch.is_contiguous() &&
+                  scratch.device() == x.device() &&
+                  (x.size(0) == 0 ||
+                   static_cast<size_t>(scratch.numel()) * 4 >=
+                       ggo_moe_route_scratch_bytes(x.size(0), static_cast<int>(num_experts))),
               "scratch must be the router's");
+}
+
+// Permute with INT8 quantisation: returns (q_sorted int8 [T*k, H], scale fp32 [T*k], slot_pos int32).
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_permute_int8(
+    const torch::Tensor& x, const torch::Tensor& topk_ids, const torch::Tensor& scratch,
+    int64_t num_experts) {
+  check_routing(x, topk_ids, scratch, num_experts);
+  const int64_t T = x.size(0), H = x.size(1), k = topk_ids.size(1);
   c10::cuda::CUDAGuard guard(x.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   auto q = empty_on(x.device(), {T * k, H}, torch::kInt8);
@@ -634,9 +642,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> moe_route
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_permute(
     const torch::Tensor& x, const torch::Tensor& topk_ids, const torch::Tensor& scratch,
     int64_t num_experts) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous(), "hidden must be 2D contiguous CUDA");
-  TORCH_CHECK(topk_ids.scalar_type() == torch::kInt32 && topk_ids.is_contiguous(),
-              "topk_ids must be contiguous int32");
+  check_routing(x, topk_ids, scratch, num_experts);
   c10::cuda::CUDAGuard guard(x.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   const int64_t T = x.size(0), H = x.size(1), k = topk_ids.size(1);
@@ -658,8 +664,13 @@ torch::Tensor moe_combine(const torch::Tensor& y_sorted, const torch::Tensor& to
               "y_sorted must be 2D contiguous CUDA");
   TORCH_CHECK(topk_weights.scalar_type() == torch::kFloat32 && topk_weights.is_contiguous(),
               "topk_weights must be contiguous fp32");
-  TORCH_CHECK(slot_pos.scalar_type() == torch::kInt32 && slot_pos.is_contiguous(),
-              "slot_pos must be contiguous int32");
+  TORCH_CHECK(topk_weights.dim() == 2 && topk_weights.device() == y_sorted.device(),
+              "topk_weights must be [T, top_k] on y_sorted's device");
+  TORCH_CHECK(y_sorted.size(0) >= topk_weights.numel(), "y_sorted must have a row per weight");
+  TORCH_CHECK(slot_pos.scalar_type() == torch::kInt32 && slot_pos.is_contiguous() &&
+                  slot_pos.numel() == topk_weights.numel() &&
+                  slot_pos.device() == y_sorted.device(),
+              "slot_pos must be contiguous int32, one per weight, on y_sorted's device");
   c10::cuda::CUDAGuard guard(y_sorted.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   const int64_t T = topk_weights.size(0), k = topk_weights.size(1), H = y_sorted.size(1);
@@ -828,10 +839,10 @@ torch::Tensor tensor_view(int64_t ptr, std::vector<int64_t> shape, torch::Dtype 
 torch::Tensor ep_dispatch(const torch::Tensor& x, const torch::Tensor& topk_ids,
                           const torch::Tensor& scratch, const torch::Tensor& counts_all,
                           int64_t rank, std::vector<int64_t> recv_ptrs,
-                          std::vector<int64_t> origin_ptrs) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous(), "hidden must be 2D contiguous CUDA");
+                          std::vector<int64_t> origin_ptrs, int64_t capacity) {
   TORCH_CHECK(counts_all.scalar_type() == torch::kInt64 && counts_all.dim() == 2 &&
                   counts_all.is_contiguous(), "counts_all must be contiguous int64 [world, E]");
+  check_routing(x, topk_ids, scratch, counts_all.size(1));
   const int world = static_cast<int>(recv_ptrs.size());
   TORCH_CHECK(world == static_cast<int>(origin_ptrs.size()) && world == counts_all.size(0) &&
                   world <= GGO_MAX_EP_RANKS, "one receive buffer and origin buffer per rank");
@@ -845,11 +856,11 @@ torch::Tensor ep_dispatch(const torch::Tensor& x, const torch::Tensor& topk_ids,
     recv[r] = reinterpret_cast<void*>(recv_ptrs[r]);
     orig[r] = reinterpret_cast<int32_t*>(origin_ptrs[r]);
   }
-  const int st = ggo_ep_dispatch(x.data_ptr(), T, H, static_cast<int>(counts_all.size(1)),
-                                 static_cast<int>(k), topk_ids.data_ptr<int32_t>(),
-                                 scratch.data_ptr(), counts_all.data_ptr<int64_t>(), world,
-                                 static_cast<int>(rank), recv.data(), orig.data(),
-                                 spos.data_ptr<int32_t>(), dtype_code(x), stream);
+  const int st = ggo_ep_dispatch_bounded(
+      x.data_ptr(), T, H, static_cast<int>(counts_all.size(1)), static_cast<int>(k),
+      topk_ids.data_ptr<int32_t>(), scratch.data_ptr(), counts_all.data_ptr<int64_t>(), world,
+      static_cast<int>(rank), capacity, recv.data(), orig.data(), spos.data_ptr<int32_t>(),
+      dtype_code(x), stream);
   check_status(st, "expert-parallel dispatch");
   return spos;
 }
@@ -998,7 +1009,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("tensor_view", &tensor_view, py::arg("ptr"), py::arg("shape"), py::arg("dtype"),
         py::arg("device"));
   m.def("ep_dispatch", &ep_dispatch, py::arg("hidden"), py::arg("topk_ids"), py::arg("scratch"),
-        py::arg("counts_all"), py::arg("rank"), py::arg("recv_ptrs"), py::arg("origin_ptrs"));
+        py::arg("counts_all"), py::arg("rank"), py::arg("recv_ptrs"), py::arg("origin_ptrs"),
+        py::arg("capacity"));
   m.def("ep_grouped_gemm", &ep_grouped_gemm, py::arg("input"), py::arg("weights"),
         py::arg("seg_counts"), py::arg("num_experts"), py::arg("swiglu"), py::arg("origin"),
         py::arg("peer_out"), py::arg("sort_by_m") = true);

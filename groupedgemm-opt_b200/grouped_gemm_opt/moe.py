@@ -144,14 +144,22 @@ def moe_router(router_logits: torch.Tensor, top_k: int,
 
 def _routing_of(routing: MoERouting, router_logits, top_k):
     """The stage outputs (ids, weights, tokens_per_expert, scratch) of a given routing, after checks
-    that it belongs to these logits' shape and device."""
+    that they are of these logits' shape and device and of the types that the stages read."""
     T, E = router_logits.shape
-    assert routing.topk_ids.shape == (T, top_k) and routing.tokens_per_expert.shape == (E,), (
-        f"routing is for {tuple(routing.topk_ids.shape)} choices over "
-        f"{routing.tokens_per_expert.numel()} experts, the layer for {(T, top_k)} over {E}")
-    assert routing.topk_ids.device == router_logits.device, "routing on another device"
-    return (routing.topk_ids, routing.topk_weights.detach(), routing.tokens_per_expert,
-            routing.scratch)
+    ids, w, tpe, scratch = (routing.topk_ids, routing.topk_weights, routing.tokens_per_expert,
+                            routing.scratch)
+    assert ids.shape == (T, top_k) and w.shape == (T, top_k) and tpe.shape == (E,), (
+        f"routing is for {tuple(ids.shape)} choices with {tuple(w.shape)} weights over "
+        f"{tpe.numel()} experts, the layer for {(T, top_k)} over {E}")
+    for name, t, dtype in (("topk_ids", ids, torch.int32), ("topk_weights", w, torch.float32),
+                           ("tokens_per_expert", tpe, torch.int64),
+                           ("scratch", scratch, torch.int32)):
+        assert t.device == router_logits.device, f"routing on another device ({name})"
+        assert t.dtype == dtype and t.is_contiguous(), f"{name} must be contiguous {dtype}"
+    # the dispatch's table: a row per 32 tokens and the experts' starts
+    assert T == 0 or scratch.numel() >= ((T + 31) // 32 + 1) * E, (
+        "the routing's scratch is not that of a router over these tokens and experts")
+    return ids, w.detach(), tpe, scratch
 
 
 class EPBuffers:
@@ -194,6 +202,8 @@ class EPBuffers:
         dev = self.device.index
         self._board_elems = int(_C.ep_board_bytes(num_experts)) // 8
         _C.tensor_view(self._own["board"], [self._board_elems], torch.int64, dev).zero_()
+        # and the origins at a row that exists: counts above the rows that arrive read unwritten ones
+        _C.tensor_view(self._own["origin"], [self.capacity], torch.int32, dev).zero_()
         torch.cuda.synchronize(self.device)
         gathered = [None] * self.world
         dist.all_gather_object(gathered, handles, group=group)
@@ -269,7 +279,7 @@ def _fused_moe_p2p(hidden, router_logits, w_gate_up, w_down, top_k, bufs: "EPBuf
     _mark(timer, "count_exchange")
     counts_all = bufs.board_counts[:world]
     slot_pos = C.ep_dispatch(hidden, ids, scratch, counts_all, rank, bufs.ptrs["recv"],
-                             bufs.ptrs["origin"])
+                             bufs.ptrs["origin"], bufs.capacity)
     _mark(timer, "dispatch")
     # phase 1: every source has delivered its rows to this rank
     C.ep_signal(boards, rank, E, 1, ep, dev)
@@ -337,7 +347,8 @@ def fused_moe(
             result scatter over NVLink inside the kernels) instead of NCCL all-to-alls.
         timer: a StageEvents that records a CUDA event after every stage (device timing).
         routing: the result of ``moe_router(router_logits, top_k)``, unchanged: the layer uses it
-            instead of routing again.
+            instead of routing again. One that does not fit in shape, type or device is refused; a
+            choice that its tables have no place for (an edited id) makes its token NaN.
 
     Returns: [T, H] = sum_j w[t,j] * down(silu(gate(x_t)) * up(x_t)) for the top-k experts.
     """

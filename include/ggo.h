@@ -301,8 +301,12 @@ int ggo_moe_permute_int8(const void* x_dev, int64_t num_tokens, int64_t hidden, 
  *   x_sorted [T*top_k, H]  the gathered hidden rows,
  *   sorted_token [T*top_k] int32, the source token of each sorted row,
  *   slot_pos [T*top_k] int32, the sorted row of (token t, slot j) at index t*top_k + j.
- * Must be called with the scratch written by ggo_moe_route on the same stream. Deterministic
- * (no atomics on positions): bit-exact against any stable counting sort. */
+ * Must be called with the ids and the scratch written by ggo_moe_route or ggo_moe_router on the same
+ * stream. Deterministic (no atomics on positions): bit-exact against any stable counting sort.
+ * A choice that the scratch has no place for (ids and scratch that do not belong together, an id
+ * outside [0, num_experts)) is dropped: slot_pos -1, which makes its token NaN in the combine. Other
+ * tokens keep their rows, and nothing outside the buffers is touched. A sorted row that no choice
+ * took is not written. */
 int ggo_moe_permute(const void* x_dev, int64_t num_tokens, int64_t hidden, int num_experts,
                     int top_k, const int32_t* topk_ids_dev, void* x_sorted_dev,
                     int32_t* sorted_token_dev, int32_t* slot_pos_dev, void* scratch_dev,
@@ -310,7 +314,8 @@ int ggo_moe_permute(const void* x_dev, int64_t num_tokens, int64_t hidden, int n
 
 /* Fused-MoE stage 4: top-k weighted combine.
  *   out[t, :] = sum_{j < top_k} topk_weights[t, j] * y_sorted[slot_pos[t*top_k + j], :]
- * accumulated in fp32 in fixed j order, rounded once to bf16/fp16. No atomics. */
+ * accumulated in fp32 in fixed j order, rounded once to bf16/fp16. No atomics. A token with a
+ * negative slot_pos (a dropped choice) gets NaN. */
 int ggo_moe_combine(const void* y_sorted_dev, const float* topk_weights_dev,
                     const int32_t* slot_pos_dev, int64_t num_tokens, int64_t hidden, int top_k,
                     void* out_dev, int dtype, cudaStream_t stream);
@@ -349,12 +354,22 @@ int ggo_ipc_free(void* ptr);
  * as mapped in this process (own buffers for r == rank). Received rows are laid out
  * expert-major, [local expert][source rank], so each local expert is one contiguous segment;
  * recv_origin holds (source rank << 28) | the row's sorted position on its source rank.
- * slot_pos_dev as in ggo_moe_permute. */
+ * slot_pos_dev and dropped choices as in ggo_moe_permute. */
 int ggo_ep_dispatch(const void* x_dev, int64_t num_tokens, int64_t hidden, int num_experts,
                     int top_k, const int32_t* topk_ids_dev, const void* scratch_dev,
                     const int64_t* counts_all_dev, int world_size, int rank,
                     void* const* recv_rows, int32_t* const* recv_origin, int32_t* slot_pos_dev,
                     int dtype, cudaStream_t stream);
+
+/* ggo_ep_dispatch with the receive buffers' rows given: a row whose place by counts_all_dev lies
+ * outside [0, capacity_rows) is dropped, so that counts which do not belong to the ids reach no
+ * memory behind a peer's buffer. */
+int ggo_ep_dispatch_bounded(const void* x_dev, int64_t num_tokens, int64_t hidden,
+                            int num_experts, int top_k, const int32_t* topk_ids_dev,
+                            const void* scratch_dev, const int64_t* counts_all_dev,
+                            int world_size, int rank, int64_t capacity_rows,
+                            void* const* recv_rows, int32_t* const* recv_origin,
+                            int32_t* slot_pos_dev, int dtype, cudaStream_t stream);
 
 /* Device-side signalling between the ranks of the fused expert-parallel path, replacing host
  * collectives. Every rank allocates a sync board of ggo_ep_board_bytes(E) bytes (zero-filled,
