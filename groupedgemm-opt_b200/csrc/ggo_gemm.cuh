@@ -163,9 +163,16 @@ __device__ __forceinline__ int block_sum(int v, int* partial) {
   return t;
 }
 
+// a + b, at most cap (a, b <= cap <= 2^31; in unsigned arithmetic nothing can wrap).
+__device__ __forceinline__ unsigned add_up_to(unsigned a, unsigned b, unsigned cap) {
+  return a + min(b, cap - a);
+}
+
 // Builds, in shared memory, the segment table every CTA needs to map a flat tile index to work:
 // clamped counts, exclusive row offsets (segment order), processing order (identity or heaviest
 // first) and exclusive tile offsets (processing order); *total_tiles_s receives the tile count.
+// Whatever the counts hold, offsets and counts end at p.rows: sums are taken up to p.rows + 1 only, and
+// a segment is cut where the rows end.
 // Called by all kThreads threads of the CTA (contains __syncthreads).
 template <int TILE_M, int OUT_BN>
 __device__ __forceinline__ void build_segment_table(const GemmParams& p, uint8_t* tiles, int* t_cnt,
@@ -185,20 +192,23 @@ __device__ __forceinline__ void build_segment_table(const GemmParams& p, uint8_t
   }
   __syncthreads();
   if (warp == 0) {  // exclusive prefix sum of rows, in segment order
-    int carry = 0;
+    const unsigned cap = static_cast<unsigned>(p.rows) + 1u;
+    unsigned carry = 0;
     for (int base = 0; base < nseg; base += 32) {
       const int s = base + lane;
-      const int v = s < nseg ? t_cnt[s] : 0;
-      int x = v;
+      unsigned x = s < nseg ? t_cnt[s] : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+        const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x = add_up_to(x, y, cap);
       }
-      if (s < nseg) t_rowoff[s] = carry + x - v;
-      carry += __shfl_sync(0xffffffffu, x, 31);
+      const unsigned before = __shfl_up_sync(0xffffffffu, x, 1);
+      if (s < nseg)
+        t_rowoff[s] = static_cast<int>(min(add_up_to(carry, lane ? before : 0u, cap), cap - 1u));
+      carry = add_up_to(carry, __shfl_sync(0xffffffffu, x, 31), cap);
     }
-    const bool bad = p.rows_is_bound ? carry > p.rows : carry != p.rows;
+    const unsigned rows = cap - 1u;
+    const bool bad = p.rows_is_bound ? carry > rows : carry != rows;
     if (lane == 0 && bad && blockIdx.x == 0) atomicCAS(err, 0, kDevCountMismatch);
   }
   if (p.split_mode) {
@@ -210,6 +220,7 @@ __device__ __forceinline__ void build_segment_table(const GemmParams& p, uint8_t
     __syncthreads();
     int mine = 0;
     for (int s = threadIdx.x; s < nseg; s += kThreads) {
+      t_cnt[s] = min(t_cnt[s], p.rows - t_rowoff[s]);
       const int r = t_cnt[s] % 256;
       mine += (r > 0 && r <= 128) ? 1 : 0;
     }
@@ -281,7 +292,13 @@ __device__ __forceinline__ void build_segment_table(const GemmParams& p, uint8_t
     int carry = 0;
     for (int base = 0; base < nseg; base += 32) {
       const int i = base + lane;
-      const int v = i < nseg ? ((t_cnt[t_order[i]] + TILE_M - 1) / TILE_M) * n_tiles : 0;
+      int v = 0;
+      if (i < nseg) {
+        const int s = t_order[i];
+        const int c = min(t_cnt[s], p.rows - t_rowoff[s]);
+        t_cnt[s] = c;
+        v = ((c + TILE_M - 1) / TILE_M) * n_tiles;
+      }
       int x = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {

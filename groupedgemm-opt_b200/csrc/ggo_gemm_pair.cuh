@@ -141,7 +141,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int carry = 0;
     for (int base = 0; base < nseg; base += 32) {
       const int s = base + lane;
-      const int v = s < nseg ? (t_cnt[s] + 127) / 128 : 0;
+      const int v = s < nseg ? (min(t_cnt[s], p.rows - t_rowoff[s]) + 127) / 128 : 0;
       int x = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {

@@ -459,30 +459,31 @@ __global__ void __launch_bounds__(256)
   __shared__ int s_blkoff[kMxMaxSegments];
   if (threadIdx.x < 32) {  // exclusive prefix sums of rows and 128-row blocks, segment order
     const int lane = threadIdx.x;
-    int carry = 0, bcarry = 0;
+    long long carry = 0, bcarry = 0;
     for (int base = 0; base < nseg; base += 32) {
       const int s = base + lane;
       long long c = s < nseg ? counts[s] : 0;
       c = c < 0 ? 0 : (c > rows ? rows : c);
-      const int v = static_cast<int>(c), b = (v + 127) / 128;
-      int xs = v, ys = b;
+      // 64-bit sums of at most nseg * rows, cut where the rows end whatever the counts hold
+      long long xs = c, ys = (c + 127) / 128;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int xu = __shfl_up_sync(0xffffffffu, xs, o);
-        const int yu = __shfl_up_sync(0xffffffffu, ys, o);
+        const long long xu = __shfl_up_sync(0xffffffffu, xs, o);
+        const long long yu = __shfl_up_sync(0xffffffffu, ys, o);
         if (lane >= o) {
           xs += xu;
           ys += yu;
         }
       }
       if (s < nseg) {
-        s_rowoff[s] = carry + xs - v;
-        s_blkoff[s] = bcarry + ys - b;
+        s_rowoff[s] = static_cast<int>(min(carry + xs - c, static_cast<long long>(rows)));
+        // (read for segments that start before the rows' end only, whose blocks are few)
+        s_blkoff[s] = static_cast<int>(bcarry + ys - (c + 127) / 128);
       }
       carry += __shfl_sync(0xffffffffu, xs, 31);
       bcarry += __shfl_sync(0xffffffffu, ys, 31);
     }
-    if (lane == 0) s_rowoff[nseg] = carry;
+    if (lane == 0) s_rowoff[nseg] = static_cast<int>(min(carry, static_cast<long long>(rows)));
   }
   __syncthreads();
   const int lane = threadIdx.x & 31;
