@@ -335,7 +335,7 @@ template <typename T16>
 int launch_permute(const void* x, int T, int H, int E, int K, const int32_t* ids,
                    const int* offsets, uint8_t* q, float* scale, int32_t* slot_pos,
                    cudaStream_t stream) {
-  const int nb = (T + kRouteTokens - 1) / kRouteTokens;
+  const int nb = (T - 1) / kRouteTokens + 1;  // T > 0; T + 31 may pass 32 bits
   const size_t smem = (2 * static_cast<size_t>(E) + kRouteTokens * K) * 4;  // at most 10 KB
   const T16* xp = static_cast<const T16*>(x);
   // Few tokens: all eight warps on one, so that every SM has a row. Else as many as hold a row of that

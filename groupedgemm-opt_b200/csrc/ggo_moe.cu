@@ -858,7 +858,7 @@ int ggo_moe_combine_checked(const void* y_sorted_dev, const float* topk_weights_
   if (T == 0) return GGO_OK;
   // About eight warps for every scheduler: below some 4700 tokens a row's columns are shared out.
   // 256 tokens x 8 slots x 7168 columns: 69 us with one warp per token, 10 us shared out.
-  const int rows8 = (T + 7) / 8, pieces = static_cast<int>((hidden / 8 + 31) / 32);
+  const int rows8 = (T - 1) / 8 + 1, pieces = static_cast<int>((hidden / 8 + 31) / 32);
   const int want = (148 * 4 + rows8 - 1) / rows8;
   const dim3 grid(rows8, want < pieces ? want : pieces);
   if (dtype == GGO_DTYPE_BF16) {

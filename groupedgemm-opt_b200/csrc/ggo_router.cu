@@ -200,7 +200,9 @@ __device__ __forceinline__ void route_block(const TL* __restrict__ logits,
   float acc[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
-  for (int t = t0 + warp; t < min(T, t0 + kTokens); t += NW) {
+  const int ntok = min(T - t0, kTokens);  // (t0 + kTokens may pass 32 bits; t0 < T)
+  for (int tl = warp; tl < ntok; tl += NW) {
+    const int t = t0 + tl;
     const TL* row = logits + static_cast<size_t>(t) * E;
     alignas(16) TL x[V];
     load_row<TL, V, VEC>(row, E, lane, x);
@@ -512,7 +514,9 @@ __global__ void __launch_bounds__(32 * kBwdWarps, bwd_blocks(V))
     cf[i] = (VEC || e < E) ? gl * coef[e] : 0.f;
   }
   __syncwarp();
-  for (int t = blockIdx.x * kBwdWarps + warp; t < T; t += gridDim.x * kBwdWarps) {
+  // unsigned: the step past the last token may lie behind 2^31
+  for (unsigned t = blockIdx.x * kBwdWarps + warp; t < static_cast<unsigned>(T);
+       t += gridDim.x * kBwdWarps) {
     const float2 st = row_stat[t];
     alignas(16) TL x[V];
     load_row<TL, V, VEC>(logits + static_cast<size_t>(t) * E, E, lane, x);
@@ -655,7 +659,7 @@ int launch_backward_as(const void* logits, const float2* stat, const int32_t* id
                        const float* coef, const float* gw, const float* gl, int T, int E, int K,
                        void* out, cudaStream_t stream) {
   const size_t smem = static_cast<size_t>(E) * kBwdWarps * 4;
-  const int want = (T + kBwdWarps - 1) / kBwdWarps;
+  const int want = (T - 1) / kBwdWarps + 1;  // T > 0; T + 7 may pass 32 bits
   const int wave = 148 * bwd_blocks(V);
   const int grid = want < wave ? want : wave;
   router_backward_kernel<TL, V, VEC><<<grid, 32 * kBwdWarps, smem, stream>>>(
