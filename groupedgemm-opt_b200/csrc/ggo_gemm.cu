@@ -663,6 +663,17 @@ int wgrad_common(const void* x, const void* dy, void* dw, const int64_t* counts,
               : launch_wgrad<128, false>(x, dy, dw, p, dev, stream);
 }
 
+// Error words are read and cleared in one step, so that none that another stream records between a
+// read and a clearing is lost.
+__global__ void take_error_kernel(GgoWorkspace* ws) { ws->taken = atomicExch(&ws->error, 0); }
+
+__global__ void collect_errors_kernel(GgoWorkspace* into, GgoWorkspace* from, int n) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  const int code = atomicExch(&from[i].error, 0);
+  if (code != 0) atomicCAS(&into->error, 0, code);
+}
+
 }  // namespace
 
 // Scratch for ggo_grouped_gemm_noalloc: one workspace (tile counter, done counter, error word) in
@@ -920,21 +931,28 @@ const char* ggo_last_cuda_error_string(void) {
   return cudaGetErrorString(static_cast<cudaError_t>(c));
 }
 
+int ggo_workspace_collect_errors(void* workspace_dev, void* others_dev, int64_t count,
+                                 cudaStream_t stream) {
+  if (!workspace_dev || (!others_dev && count > 0) || count < 0) return GGO_ERR_INVALID_ARG;
+  if (count > (1 << 30)) return GGO_ERR_SHAPE;
+  if (count == 0) return GGO_OK;
+  const int n = static_cast<int>(count);
+  ggo::collect_errors_kernel<<<(n + 255) / 256, 256, 0, stream>>>(
+      static_cast<ggo::GgoWorkspace*>(workspace_dev), static_cast<ggo::GgoWorkspace*>(others_dev),
+      n);
+  return ggo::check_launch();
+}
+
 int ggo_workspace_error(void* workspace_dev, cudaStream_t stream, int* status_out) {
   if (!workspace_dev || !status_out) return GGO_ERR_INVALID_ARG;
   int code = 0;
   auto* ws = static_cast<ggo::GgoWorkspace*>(workspace_dev);
-  if (cudaMemcpyAsync(&code, &ws->error, sizeof(int), cudaMemcpyDeviceToHost, stream) !=
+  ggo::take_error_kernel<<<1, 1, 0, stream>>>(ws);
+  if (int st = ggo::check_launch()) return st;
+  if (cudaMemcpyAsync(&code, &ws->taken, sizeof(int), cudaMemcpyDeviceToHost, stream) !=
           cudaSuccess ||
       cudaStreamSynchronize(stream) != cudaSuccess)
     return GGO_ERR_CUDA;
-  if (code != 0) {
-    const int zero = 0;
-    if (cudaMemcpyAsync(&ws->error, &zero, sizeof(int), cudaMemcpyHostToDevice, stream) !=
-            cudaSuccess ||
-        cudaStreamSynchronize(stream) != cudaSuccess)
-      return GGO_ERR_CUDA;
-  }
   *status_out = ggo::device_error_to_status(code);
   return GGO_OK;
 }

@@ -73,7 +73,8 @@ struct GgoWorkspace {
   int tile_counter;
   int done_counter;
   int error;
-  int pad[61];
+  int taken;  // the error that was last read (and cleared)
+  int pad[60];
 };
 
 struct GemmParams {

@@ -43,66 +43,116 @@ bool capturing(cudaStream_t stream) {
   return st != cudaStreamCaptureStatusNone;
 }
 
+// Zero-filled device memory that outlives any graph. While `stream` is being captured it must neither
+// come from the graph's memory pool nor be zeroed by a node of the graph: it is made on a stream that
+// is not being captured, and waited for.
+torch::Tensor lasting_zeros(const torch::Device& dev, cudaStream_t stream, int64_t bytes) {
+  const auto opts = torch::TensorOptions().dtype(torch::kUInt8).device(dev);
+  if (!capturing(stream)) return torch::zeros({bytes}, opts);
+  c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+  c10::cuda::CUDAStream side = c10::cuda::getStreamFromPool(false, dev.index());
+  for (int i = 0; i < 64 && capturing(side); ++i)
+    side = c10::cuda::getStreamFromPool(false, dev.index());
+  c10::cuda::CUDAStreamGuard on_side(side);
+  torch::Tensor t = torch::zeros({bytes}, opts);
+  TORCH_CHECK(cudaStreamSynchronize(side) == cudaSuccess, "workspace set-up");
+  return t;
+}
+
 // One zero-initialised workspace per (device, stream); kept for the life of the process.
 std::mutex g_ws_mu;
 std::map<std::pair<int, cudaStream_t>, torch::Tensor> g_ws;
 
-void* workspace_for(const torch::Device& dev, cudaStream_t stream, bool in_capture) {
+void* workspace_for(const torch::Device& dev, cudaStream_t stream) {
   std::lock_guard<std::mutex> lk(g_ws_mu);
   auto key = std::make_pair(static_cast<int>(dev.index()), stream);
   auto it = g_ws.find(key);
-  if (it == g_ws.end()) {
-    const auto opts = torch::TensorOptions().dtype(torch::kUInt8).device(dev);
-    const int64_t bytes = static_cast<int64_t>(ggo_workspace_size());
-    torch::Tensor t;
-    if (in_capture) {
-      // The first call on this stream is a captured one. The workspace outlives the graph and is
-      // used outside it too, so it must neither come from the graph's memory pool nor be zeroed by
-      // a node of the graph: make it on a stream that is not being captured, and wait for it.
-      c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
-      c10::cuda::CUDAStream side = c10::cuda::getStreamFromPool(false, dev.index());
-      for (int i = 0; i < 64 && capturing(side); ++i)
-        side = c10::cuda::getStreamFromPool(false, dev.index());
-      c10::cuda::CUDAStreamGuard on_side(side);
-      t = torch::zeros({bytes}, opts);
-      TORCH_CHECK(cudaStreamSynchronize(side) == cudaSuccess, "workspace set-up");
-    } else {
-      t = torch::zeros({bytes}, opts);
-    }
-    it = g_ws.emplace(key, t).first;
-  }
+  if (it == g_ws.end())
+    it = g_ws.emplace(key, lasting_zeros(dev, stream, static_cast<int64_t>(ggo_workspace_size())))
+             .first;
   return it->second.data_ptr();
 }
 
-void* workspace_for(const torch::Device& dev, cudaStream_t stream) {
-  return workspace_for(dev, stream, capturing(stream));
+// Workspaces of captured calls, in chunks that last for the life of the process. A captured call takes
+// one and its graph gives it back when it (and what was instantiated from it) is gone. The kernels
+// leave the counters at zero, so a workspace needs no node that zeroes it; its error word stays here
+// too, where workspace_error finds it.
+struct CapturedWorkspaces {
+  static constexpr int64_t kChunk = 64;
+  std::mutex mu;
+  std::map<int, std::vector<torch::Tensor>> chunks;  // by device
+  std::map<int, std::vector<char*>> unused;
+};
+
+CapturedWorkspaces& captured_workspaces() {
+  static auto* all = new CapturedWorkspaces;  // never destroyed: graphs may go after it
+  return *all;
 }
 
-// Stands for "any stream" among the keys of the workspaces: the one whose error word takes the errors
-// of captured calls, which may be replayed on any stream.
-cudaStream_t captured_key() { return reinterpret_cast<cudaStream_t>(&g_ws_mu); }
-
-// Workspace of one call. Eager calls share the stream's workspace (they run in stream order). A
-// captured call gets a zero-filled one of its own inside the graph, so that replays of several
-// graphs may overlap each other and eager calls; its device errors go to the device's word for
-// captured calls, which workspace_error reads too.
-struct CallWorkspace {
-  torch::Tensor own;  // captured calls only
-  void* ws = nullptr;
-  int* err = nullptr;
-
-  CallWorkspace(const torch::Device& dev, cudaStream_t stream) {
-    if (!capturing(stream)) {
-      ws = workspace_for(dev, stream);
-      err = ggo_workspace_error_word(ws);
-      return;
-    }
-    err = ggo_workspace_error_word(workspace_for(dev, captured_key(), true));
-    own = torch::zeros({static_cast<int64_t>(ggo_workspace_size())},
-                       torch::TensorOptions().dtype(torch::kUInt8).device(dev));
-    ws = own.data_ptr();
-  }
+struct CapturedLease {
+  int dev;
+  char* ws;
 };
+
+void end_lease(void* p) {
+  auto* lease = static_cast<CapturedLease*>(p);
+  auto& all = captured_workspaces();
+  {
+    std::lock_guard<std::mutex> lk(all.mu);
+    all.unused[lease->dev].push_back(lease->ws);
+  }
+  delete lease;
+}
+
+void* captured_workspace(const torch::Device& dev, cudaStream_t stream) {
+  auto& all = captured_workspaces();
+  auto* lease = new CapturedLease{static_cast<int>(dev.index()), nullptr};
+  {
+    std::lock_guard<std::mutex> lk(all.mu);
+    auto& unused = all.unused[lease->dev];
+    if (unused.empty()) {
+      const int64_t size = static_cast<int64_t>(ggo_workspace_size());
+      auto chunk = lasting_zeros(dev, stream, CapturedWorkspaces::kChunk * size);
+      unused.reserve(unused.size() + CapturedWorkspaces::kChunk);
+      for (int64_t i = CapturedWorkspaces::kChunk; i-- > 0;)
+        unused.push_back(reinterpret_cast<char*>(chunk.data_ptr<uint8_t>()) + i * size);
+      all.chunks[lease->dev].push_back(std::move(chunk));
+    }
+    lease->ws = unused.back();
+    unused.pop_back();
+  }
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  cudaGraph_t graph = nullptr;
+  cudaUserObject_t owner = nullptr;
+  void* ws = lease->ws;
+  const bool made =
+      cudaStreamGetCaptureInfo(stream, &st, nullptr, &graph, nullptr, nullptr) == cudaSuccess &&
+      st == cudaStreamCaptureStatusActive &&
+      cudaUserObjectCreate(&owner, lease, end_lease, 1, cudaUserObjectNoDestructorSync) ==
+          cudaSuccess;
+  if (!made) end_lease(lease);
+  TORCH_CHECK(made, "workspace of a captured call");
+  if (cudaGraphRetainUserObject(graph, owner, 1, cudaGraphUserObjectMove) != cudaSuccess) {
+    cudaUserObjectRelease(owner, 1);
+    TORCH_CHECK(false, "workspace of a captured call");
+  }
+  return ws;
+}
+
+// (in use, made) on one device, for tests
+std::tuple<int64_t, int64_t> captured_workspace_counts(int64_t device) {
+  auto& all = captured_workspaces();
+  std::lock_guard<std::mutex> lk(all.mu);
+  const int dev = static_cast<int>(device);
+  const int64_t made = static_cast<int64_t>(all.chunks[dev].size()) * CapturedWorkspaces::kChunk;
+  return {made - static_cast<int64_t>(all.unused[dev].size()), made};
+}
+
+// Workspace of one product. Eager calls share the stream's (they run in stream order). A captured call
+// has one of its own, so that replays of several graphs may overlap each other and eager calls.
+void* call_workspace(const torch::Device& dev, cudaStream_t stream) {
+  return capturing(stream) ? captured_workspace(dev, stream) : workspace_for(dev, stream);
+}
 
 torch::Tensor counts_on_device(const torch::Tensor& counts, const torch::Device& dev) {
   auto c = counts.to(torch::kInt64);
@@ -140,7 +190,7 @@ torch::Tensor grouped_gemm_segments(const torch::Tensor& input, const torch::Ten
   const int st = ggo_grouped_gemm_segments(
       input.data_ptr(), weights.data_ptr(), out.data_ptr(), c.data_ptr<int64_t>(),
       static_cast<int>(c.size(0)), static_cast<int>(num_experts), T, N, K, dtype_code(input),
-      static_cast<int>(tile_config), sort_by_m ? 1 : 0, workspace_for(input.device(), stream),
+      static_cast<int>(tile_config), sort_by_m ? 1 : 0, call_workspace(input.device(), stream),
       stream);
   check_status(st, "grouped GEMM");
   return out;
@@ -177,7 +227,7 @@ torch::Tensor grouped_gemm_dgrad(const torch::Tensor& dy, const torch::Tensor& w
   const int st = ggo_grouped_gemm_dgrad(
       dy.data_ptr(), weights.data_ptr(), dx.data_ptr(), c.data_ptr<int64_t>(),
       static_cast<int>(weights.size(0)), T, N, K, dtype_code(dy), static_cast<int>(tile_config),
-      sort_by_m ? 1 : 0, workspace_for(dy.device(), stream), stream);
+      sort_by_m ? 1 : 0, call_workspace(dy.device(), stream), stream);
   check_status(st, "grouped GEMM dgrad");
   return dx;
 }
@@ -199,7 +249,7 @@ torch::Tensor grouped_gemm_wgrad(const torch::Tensor& x, const torch::Tensor& dy
   const int st = ggo_grouped_gemm_wgrad(x.data_ptr(), dy.data_ptr(), dw.data_ptr(),
                                         c.data_ptr<int64_t>(), static_cast<int>(E), T, N, K,
                                         dtype_code(x), sort_by_m ? 1 : 0,
-                                        workspace_for(x.device(), stream), stream);
+                                        call_workspace(x.device(), stream), stream);
   check_status(st, "grouped GEMM wgrad");
   return dw;
 }
@@ -245,7 +295,7 @@ torch::Tensor grouped_gemm_fp8(const torch::Tensor& a_q, const torch::Tensor& a_
   const int st = ggo_grouped_gemm_fp8(
       a_q.data_ptr(), a_scale.data_ptr<float>(), w_q.data_ptr(), w_scale.data_ptr<float>(),
       out.data_ptr(), c.data_ptr<int64_t>(), static_cast<int>(E), T, N, K,
-      static_cast<int>(tile_config), sort_by_m ? 1 : 0, workspace_for(a_q.device(), stream),
+      static_cast<int>(tile_config), sort_by_m ? 1 : 0, call_workspace(a_q.device(), stream),
       stream);
   check_status(st, "fp8 grouped GEMM");
   return out;
@@ -277,7 +327,7 @@ torch::Tensor grouped_gemm_swiglu_fp8(const torch::Tensor& x_q, const torch::Ten
       x_q.data_ptr(), x_scale.data_ptr<float>(), w_q.data_ptr(), w_scale.data_ptr<float>(),
       h.data_ptr(), c.data_ptr<int64_t>(), static_cast<int>(c.size(0)),
       static_cast<int>(num_experts), T, F, K, sort_by_m ? 1 : 0,
-      workspace_for(x_q.device(), stream), stream);
+      call_workspace(x_q.device(), stream), stream);
   check_status(st, "fp8 gate/up SwiGLU grouped GEMM");
   return h;
 }
@@ -336,7 +386,7 @@ torch::Tensor grouped_gemm_mxfp8(const torch::Tensor& a_q, const torch::Tensor& 
   const int st = ggo_grouped_gemm_mxfp8(
       a_q.data_ptr(), a_sf.data_ptr(), w_q.data_ptr(), w_sf.data_ptr(), out.data_ptr(),
       c.data_ptr<int64_t>(), static_cast<int>(c.numel()), static_cast<int>(num_experts), T, N, K,
-      sort_by_m ? 1 : 0, workspace_for(a_q.device(), stream), stream);
+      sort_by_m ? 1 : 0, call_workspace(a_q.device(), stream), stream);
   check_status(st, "mxfp8 grouped GEMM");
   return out;
 }
@@ -358,7 +408,7 @@ torch::Tensor grouped_gemm_swiglu_mxfp8(const torch::Tensor& x_q, const torch::T
   const int st = ggo_grouped_gemm_swiglu_mxfp8(
       x_q.data_ptr(), x_sf.data_ptr(), w_q.data_ptr(), w_sf.data_ptr(), h.data_ptr(),
       c.data_ptr<int64_t>(), static_cast<int>(c.numel()), static_cast<int>(num_experts), T, F, K,
-      sort_by_m ? 1 : 0, workspace_for(x_q.device(), stream), stream);
+      sort_by_m ? 1 : 0, call_workspace(x_q.device(), stream), stream);
   check_status(st, "mxfp8 gate/up SwiGLU grouped GEMM");
   return h;
 }
@@ -377,7 +427,7 @@ torch::Tensor grouped_gemm_swiglu(const torch::Tensor& x, const torch::Tensor& w
   const int st = ggo_grouped_gemm_swiglu(
       x.data_ptr(), w_gate_up.data_ptr(), h.data_ptr(), c.data_ptr<int64_t>(),
       static_cast<int>(c.size(0)), static_cast<int>(num_experts), T, F, K, dtype_code(x),
-      sort_by_m ? 1 : 0, workspace_for(x.device(), stream), stream);
+      sort_by_m ? 1 : 0, call_workspace(x.device(), stream), stream);
   check_status(st, "gate/up SwiGLU grouped GEMM");
   return h;
 }
@@ -448,12 +498,11 @@ torch::Tensor grouped_gemm_int8(const torch::Tensor& a_q, const torch::Tensor& a
   auto out = empty_on(a_q.device(), {T, N}, out_dtype);
   if (T == 0) return out;
   auto c = counts_for_call(counts, a_q.device(), stream);
-  CallWorkspace ws(a_q.device(), stream);
   const int st = ggo_grouped_gemm_int8(
       a_q.data_ptr(), a_scale.data_ptr<float>(), w_q.data_ptr(), w_scale.data_ptr<float>(),
       out.data_ptr(), c.data_ptr<int64_t>(), static_cast<int>(E), static_cast<int>(E), T, N, K,
-      dtype_code(out), swiglu ? 1 : 0, static_cast<int>(tile_config), sort_by_m ? 1 : 0, ws.ws,
-      ws.err, stream);
+      dtype_code(out), swiglu ? 1 : 0, static_cast<int>(tile_config), sort_by_m ? 1 : 0,
+      call_workspace(a_q.device(), stream), nullptr, stream);
   check_status(st, swiglu ? "int8 gate/up SwiGLU grouped GEMM" : "int8 grouped GEMM");
   return out;
 }
@@ -684,25 +733,23 @@ torch::Tensor moe_combine(const torch::Tensor& y_sorted, const torch::Tensor& to
   return out;
 }
 
-// Reads and clears the device-side error word of the current stream's workspace, and that of captured
+// Reads and clears the device-side error word of the current stream's workspace and those of captured
 // calls (synchronises).
 int64_t workspace_error(int64_t device) {
   c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   const torch::Device dev(torch::kCUDA, static_cast<c10::DeviceIndex>(device));
-  int code = 0;
-  check_status(ggo_workspace_error(workspace_for(dev, stream), stream, &code),
-               "workspace error read");
-  if (code == 0) {  // and the word of captured calls, if there have been any
-    void* captured = nullptr;
-    {
-      std::lock_guard<std::mutex> lk(g_ws_mu);
-      auto it = g_ws.find(std::make_pair(static_cast<int>(device), captured_key()));
-      if (it != g_ws.end()) captured = it->second.data_ptr();
-    }
-    if (captured)
-      check_status(ggo_workspace_error(captured, stream, &code), "workspace error read");
+  void* ws = workspace_for(dev, stream);
+  {
+    auto& all = captured_workspaces();
+    std::lock_guard<std::mutex> lk(all.mu);
+    for (const auto& chunk : all.chunks[static_cast<int>(device)])
+      check_status(ggo_workspace_collect_errors(ws, chunk.data_ptr(), CapturedWorkspaces::kChunk,
+                                                stream),
+                   "workspace error read");
   }
+  int code = 0;
+  check_status(ggo_workspace_error(ws, stream, &code), "workspace error read");
   return code;
 }
 
@@ -758,6 +805,7 @@ torch::Tensor grouped_gemm_host(const torch::Tensor& input, const torch::Tensor&
   auto d_x = torch::empty({T, K}, dopt);
   auto d_y = torch::empty({T, N}, dopt);
   auto d_c = torch::empty({E}, torch::TensorOptions().dtype(torch::kInt64).device(weights.device()));
+  void* ws = call_workspace(weights.device(), cur);
   std::vector<cudaEvent_t> evs;
   auto event = [&](cudaStream_t s) {
     cudaEvent_t ev;
@@ -773,7 +821,6 @@ torch::Tensor grouped_gemm_host(const torch::Tensor& input, const torch::Tensor&
   const int64_t nch = std::max<int64_t>(1, chunks);
   int64_t e_begin = 0, row = 0;
   const int dt = dtype_code(input);
-  void* ws = workspace_for(weights.device(), s_mm);
   for (int64_t ch = 0; ch < nch && e_begin < E; ++ch) {
     // next group: experts until the group holds about T / nch rows (the last takes the rest)
     int64_t e_end = e_begin, rows = 0;
@@ -891,6 +938,7 @@ torch::Tensor ep_grouped_gemm(const torch::Tensor& input, const torch::Tensor& w
   }
   if (cap == 0) return out;
   auto c = counts_on_device(seg_counts, input.device());
+  // the stream's workspace: the layer's checked combine reads its error word
   const int st = ggo_ep_grouped_gemm(
       input.data_ptr(), weights.data_ptr(), org ? nullptr : out.data_ptr(),
       c.data_ptr<int64_t>(), static_cast<int>(c.size(0)), static_cast<int>(num_experts), cap, N,
@@ -990,6 +1038,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("moe_combine", &moe_combine, py::arg("y_sorted"), py::arg("topk_weights"),
         py::arg("slot_pos"), py::arg("checked") = false);
   m.def("workspace_error", &workspace_error, py::arg("device") = 0);
+  m.def("captured_workspaces", &captured_workspace_counts, py::arg("device") = 0);
   m.def("abi_version", []() { return ggo_version(); });
   m.def("kernel_launches", []() { return static_cast<int64_t>(ggo_kernel_launches()); });
   m.def("grouped_gemm_host", &grouped_gemm_host, py::arg("input"), py::arg("weights"),

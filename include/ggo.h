@@ -426,9 +426,16 @@ int ggo_grouped_gemm_noalloc(const void* input_dev, const void* weights_dev, voi
                              int64_t total_tokens, int64_t N, int64_t K, int dtype,
                              int tile_config, int sort_by_m, cudaStream_t stream);
 
-/* Reads (and clears) the sticky device error of a workspace. Synchronises `stream`.
+/* Reads (and clears, in one step) the sticky device error of a workspace. Synchronises `stream`.
  * Writes GGO_OK or a GGO_ERR_* code to *status_out. */
 int ggo_workspace_error(void* workspace_dev, cudaStream_t stream, int* status_out);
+
+/* Moves the device errors of `count` workspaces that lie one after the other (ggo_workspace_size()
+ * bytes each) into the error of workspace_dev, unless that holds one already. Asynchronous. For
+ * programs that give captured calls workspaces of their own, so that graphs may be replayed at the
+ * same time, and ask after all of them at once. */
+int ggo_workspace_collect_errors(void* workspace_dev, void* others_dev, int64_t count,
+                                 cudaStream_t stream);
 
 #ifdef __cplusplus
 }
