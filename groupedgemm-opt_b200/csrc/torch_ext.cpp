@@ -734,7 +734,8 @@ torch::Tensor moe_combine(const torch::Tensor& y_sorted, const torch::Tensor& to
 }
 
 // Reads and clears the device-side error word of the current stream's workspace and those of captured
-// calls (synchronises).
+// calls. Synchronises the current stream or, as replays may run on any stream, the device if products
+// have been captured.
 int64_t workspace_error(int64_t device) {
   c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
@@ -742,8 +743,16 @@ int64_t workspace_error(int64_t device) {
   void* ws = workspace_for(dev, stream);
   {
     auto& all = captured_workspaces();
-    std::lock_guard<std::mutex> lk(all.mu);
-    for (const auto& chunk : all.chunks[static_cast<int>(device)])
+    std::vector<torch::Tensor> chunks;
+    {
+      std::lock_guard<std::mutex> lk(all.mu);
+      chunks = all.chunks[static_cast<int>(device)];
+    }
+    if (!chunks.empty()) {
+      const cudaError_t e = cudaDeviceSynchronize();
+      TORCH_CHECK(e == cudaSuccess, "workspace error read failed: ", cudaGetErrorString(e));
+    }
+    for (const auto& chunk : chunks)
       check_status(ggo_workspace_collect_errors(ws, chunk.data_ptr(), CapturedWorkspaces::kChunk,
                                                 stream),
                    "workspace error read");

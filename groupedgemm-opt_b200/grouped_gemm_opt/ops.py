@@ -106,8 +106,10 @@ def grouped_gemm_opt(
 
 def check_device_errors(device: int = 0) -> None:
     """Synchronises and raises RuntimeError if a kernel on the current stream recorded an error
-    (count mismatch with GPU counts, negative count, or an expired bounded wait), or an INT8 product
-    replayed from a CUDA graph did."""
+    (count mismatch with GPU counts, negative count, or an expired bounded wait), or a product
+    replayed from a CUDA graph on any stream did. Once products have been captured on ``device`` it
+    synchronises the whole device, else the current stream; not to be called while a graph is
+    being captured."""
     code = int(_C.workspace_error(device))
     if code:
         raise RuntimeError(f"grouped_gemm_opt device error code {code}")
