@@ -15,6 +15,7 @@
 
 #include "ggo.h"
 #include "ggo_internal.h"
+#include "ggo_order.cuh"
 
 namespace ggo {
 namespace {
@@ -25,18 +26,8 @@ constexpr int kRouteThreads = 256;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopK = 16;
 
-// Monotone float -> uint32 map (larger float -> larger key); 0 is below every real key and marks
-// an expert already chosen.
-__device__ __forceinline__ uint32_t fkey(float f) {
-  const uint32_t b = __float_as_uint(f);
-  const uint32_t k = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-  return k == 0 ? 1u : k;
-}
-__device__ __forceinline__ float fkey_inv(uint32_t k) {
-  const uint32_t b = (k & 0x80000000u) ? (k & 0x7fffffffu) : ~k;
-  return __uint_as_float(b);
-}
-
+// Top-k in the order of order_key (ties to the lower expert; key 0 marks an expert already chosen) and
+// the softmax over the chosen logits; weights 0 for a row of nothing but -inf.
 // grid = ceil(T / kRouteTokens); dynamic smem = (8 warps * E + E) * 4 bytes.
 __global__ void __launch_bounds__(kRouteThreads)
     route_kernel(const float* __restrict__ logits, int T, int E, int K,
@@ -53,7 +44,7 @@ __global__ void __launch_bounds__(kRouteThreads)
     const int t = t0 + tl;
     if (t >= T) break;
     const float* row = logits + static_cast<size_t>(t) * E;
-    for (int e = lane; e < E; e += 32) keys[e] = fkey(row[e]);
+    for (int e = lane; e < E; e += 32) keys[e] = order_key(row[e]);
     __syncwarp();
     float vals[kMaxTopK];
     int ids[kMaxTopK];
@@ -72,19 +63,20 @@ __global__ void __launch_bounds__(kRouteThreads)
       }
       const int id = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best & 0xffffffffu));
       ids[j] = id;
-      vals[j] = fkey_inv(static_cast<uint32_t>(best >> 32));
+      vals[j] = order_value(static_cast<uint32_t>(best >> 32));
       __syncwarp();
       if (lane == 0) keys[id] = 0;
       __syncwarp();
     }
     if (lane == 0) {
       // softmax over the selected logits (vals[0] is the maximum)
+      const bool live = vals[0] != -INFINITY;
       float s = 0.f, ex[kMaxTopK];
       for (int j = 0; j < K; ++j) {
-        ex[j] = expf(vals[j] - vals[0]);
+        ex[j] = live ? expf(vals[j] - vals[0]) : 0.f;
         s += ex[j];
       }
-      const float inv = 1.0f / s;
+      const float inv = live ? 1.0f / s : 0.f;
       for (int j = 0; j < K; ++j) {
         topk_ids[static_cast<size_t>(t) * K + j] = ids[j];
         topk_w[static_cast<size_t>(t) * K + j] = ex[j] * inv;

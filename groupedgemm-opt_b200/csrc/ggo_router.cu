@@ -18,6 +18,7 @@
 
 #include "ggo.h"
 #include "ggo_internal.h"
+#include "ggo_order.cuh"
 
 namespace ggo {
 namespace {
@@ -26,14 +27,6 @@ constexpr int kTokens = 32;    // tokens per block: the granularity of the dispa
 constexpr int kMaxE = 1024;
 constexpr int kMaxK = 16;
 constexpr unsigned kAll = 0xffffffffu;
-
-// Monotone float -> uint32 (larger float -> larger key). -0 counts as +0 and NaN as the largest, so
-// that equal floats have equal keys; no float has key 0.
-__device__ __forceinline__ uint32_t order_key(float f) {
-  if (f != f) return 0xffffffffu;
-  const uint32_t b = __float_as_uint(f + 0.0f);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
 
 // A logit's key and its expert in one word, larger for larger logits and, among equal keys, for
 // lower experts, so that a plain maximum chooses. The 16-bit types' keys are whole (upper half);

@@ -5,8 +5,9 @@ The reference's fused-MoE entry point (grouped_gemm_opt/triton_fused_moe.py:104-
 grouped GEMM over pre-sorted rows; this module is the complete layer that its name promises.
 
 Conventions (fixed here, relied on by the kernels and the tests):
-  * router: top-k of the fp32 logits, ties to the lower expert index, softmax over the k selected
-    logits (Mixtral style), weights kept in fp32.
+  * router: top-k of the fp32 logits, ties (signed zeros among them) to the lower expert index, NaN
+    above +inf, softmax over the k selected logits (Mixtral style), weights kept in fp32, 0 for a
+    token whose logits are all -inf.
   * sorted order: expert-major, then token index (a stable counting sort).
   * w_gate_up [E, 2F, H]: rows 0..F-1 are the gate projection, rows F..2F-1 the up projection.
   * w_down [E, H, F].

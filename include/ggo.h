@@ -249,9 +249,10 @@ int ggo_grouped_gemm_swiglu(const void* x_dev, const void* w_gate_up_dev, void* 
                             int num_experts, int64_t total_tokens, int64_t F, int64_t K, int dtype,
                             int sort_by_m, void* workspace_dev, cudaStream_t stream);
 
-/* Fused-MoE stage 1a: router. For every token t: the top_k largest logits (ties -> lower expert
- * index), softmax over those k values (fp32), written as topk_ids [T, top_k] int32 and
- * topk_weights [T, top_k] fp32, in descending-logit order. Also writes tokens_per_expert [E]
+/* Fused-MoE stage 1a: router. For every token t: the top_k largest logits (ties, signed zeros among
+ * them, -> lower expert index; NaN ranks above +inf), softmax over those k values (fp32), written as
+ * topk_ids [T, top_k] int32 and topk_weights [T, top_k] fp32, in descending-logit order. A token whose
+ * logits are all -inf gets the weights 0. Also writes tokens_per_expert [E]
  * int64. logits fp32 [T, E]. E <= 1024, top_k <= 16, top_k <= E.
  * block_counts_dev needs ggo_moe_route_scratch_bytes(T, E) bytes. No reference counterpart. */
 size_t ggo_moe_route_scratch_bytes(int64_t num_tokens, int num_experts);

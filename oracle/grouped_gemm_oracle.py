@@ -121,14 +121,19 @@ def dirichlet_counts(total_tokens: int, num_experts: int, alpha: float = 0.5, se
 
 # ----------------------------------------------------------------------------- fused MoE
 def route(logits: np.ndarray, top_k: int):
-    """Top-k (ties -> lower index) then softmax over the selected logits, fp32.
+    """Top-k (ties -> lower index, signed zeros among them; NaN ranks above +inf) then softmax over the
+    selected logits, fp32; weights 0 for a row of nothing but -inf.
     Returns ids int32 [T,k], weights fp32 [T,k], tokens_per_expert int64 [E]."""
     lg = np.asarray(logits, dtype=np.float32)
     T, E = lg.shape
-    order = np.argsort(-lg, axis=1, kind="stable")[:, :top_k]
+    nan = np.isnan(lg)
+    # by (not NaN, -logit), then index; -lg of a NaN is replaced, as it would sort last
+    order = np.lexsort((np.where(nan, 0, -lg), ~nan), axis=1)[:, :top_k]
     vals = np.take_along_axis(lg, order, axis=1)
-    ex = np.exp(vals - vals[:, :1])
-    w = (ex / ex.sum(axis=1, keepdims=True)).astype(np.float32)
+    live = vals[:, :1] != -np.inf
+    with np.errstate(invalid="ignore"):
+        ex = np.where(live, np.exp(np.where(live, vals - vals[:, :1], 0)), 0).astype(np.float32)
+    w = (ex / np.where(live, ex.sum(axis=1, keepdims=True), 1)).astype(np.float32)
     tpe = np.bincount(order.reshape(-1), minlength=E).astype(np.int64)
     return order.astype(np.int32), w, tpe
 
