@@ -432,15 +432,21 @@ __device__ __forceinline__ float acc_to_float(uint32_t v) {
 }
 
 // silu(gate) * up of two accumulator words under their scales. The integer path divides by
-// multiplying with the hardware reciprocal (within 2 ulp, far below the rounding to 16 bits that
-// follows).
+// multiplying with the hardware reciprocal, within 2 ulp for divisors up to 2^126 (far below the
+// rounding to 16 bits that follows) and 0 beyond. Gates below -64, where 1 + e^-g is e^-g, take
+// g e^g u instead, as (g e^(g/2)) (u e^(g/2)): no factor leaves the normal numbers before the result
+// does.
 template <bool I8>
 __device__ __forceinline__ float scaled_silu_mul(uint32_t g, uint32_t u, float rs, float cg,
                                                  float cu) {
   const float gv = acc_to_float<I8>(g) * rs * cg;
   const float uv = acc_to_float<I8>(u) * rs * cu;
-  const float d = 1.0f + __expf(-gv);
-  return (I8 ? __fdividef(gv, d) : gv / d) * uv;
+  if (I8) {
+    const bool far = gv < -64.f;
+    const float e = __expf(far ? 0.5f * gv : -gv);
+    return far ? (gv * e) * (uv * e) : __fdividef(gv, 1.0f + e) * uv;
+  }
+  return gv / (1.0f + __expf(-gv)) * uv;
 }
 
 // Whether 32 column scales can be read as eight 16-byte words (warp-uniform): all of them exist and
