@@ -626,7 +626,7 @@ int dispatch_common(const void* x, int64_t num_tokens, int64_t hidden, int E, in
                     const int32_t* ids, const void* scratch, const int64_t* counts_all, int world,
                     int rank, int64_t capacity, void* const* recv, int32_t* const* origin, int32_t* stok,
                     int32_t* spos, int dtype, cudaStream_t stream) {
-  if (!x || !ids || !spos || !scratch) return GGO_ERR_INVALID_ARG;
+  if (num_tokens > 0 && (!x || !ids || !spos || !scratch)) return GGO_ERR_INVALID_ARG;
   if (num_tokens < 0 || hidden <= 0 || E <= 0 || E > kMaxExperts || K <= 0 || K > kMaxTopK)
     return GGO_ERR_INVALID_ARG;
   if (dtype != GGO_DTYPE_BF16 && dtype != GGO_DTYPE_FP16) return GGO_ERR_DTYPE;
@@ -662,7 +662,8 @@ size_t ggo_moe_route_scratch_bytes(int64_t num_tokens, int num_experts) {
 int ggo_moe_route(const float* logits_dev, int64_t num_tokens, int num_experts, int top_k,
                   int32_t* topk_ids_dev, float* topk_weights_dev,
                   int64_t* tokens_per_expert_dev, void* scratch_dev, cudaStream_t stream) {
-  if (!logits_dev || !topk_ids_dev || !topk_weights_dev || !tokens_per_expert_dev || !scratch_dev)
+  if (!tokens_per_expert_dev || !scratch_dev ||
+      (num_tokens != 0 && (!logits_dev || !topk_ids_dev || !topk_weights_dev)))
     return GGO_ERR_INVALID_ARG;
   if (num_tokens < 0 || num_experts <= 0 || num_experts > ggo::kMaxExperts || top_k <= 0 ||
       top_k > ggo::kMaxTopK || top_k > num_experts)
@@ -688,7 +689,7 @@ int ggo_moe_permute(const void* x_dev, int64_t num_tokens, int64_t hidden, int n
                     int top_k, const int32_t* topk_ids_dev, void* x_sorted_dev,
                     int32_t* sorted_token_dev, int32_t* slot_pos_dev, void* scratch_dev,
                     int dtype, cudaStream_t stream) {
-  if (!x_sorted_dev || !sorted_token_dev) return GGO_ERR_INVALID_ARG;
+  if (num_tokens != 0 && (!x_sorted_dev || !sorted_token_dev)) return GGO_ERR_INVALID_ARG;
   void* recv[1] = {x_sorted_dev};
   int32_t* origin[1] = {nullptr};
   return ggo::dispatch_common(x_dev, num_tokens, hidden, num_experts, top_k, topk_ids_dev,
@@ -725,7 +726,8 @@ int ggo_ep_dispatch(const void* x_dev, int64_t num_tokens, int64_t hidden, int n
 
 int ggo_quantize_fp8_rows(const void* x_dev, int64_t rows, int64_t cols, int dtype, void* q_dev,
                           float* scale_dev, cudaStream_t stream) {
-  if (!x_dev || !q_dev || !scale_dev || rows < 0 || cols <= 0) return GGO_ERR_INVALID_ARG;
+  if (rows < 0 || cols <= 0 || (rows > 0 && (!x_dev || !q_dev || !scale_dev)))
+    return GGO_ERR_INVALID_ARG;
   if (dtype != GGO_DTYPE_BF16 && dtype != GGO_DTYPE_FP16) return GGO_ERR_DTYPE;
   if (cols % 16 || !ggo::aligned16(x_dev) || !ggo::aligned16(q_dev)) return GGO_ERR_ALIGNMENT;
   if (rows > INT32_MAX || cols > INT32_MAX) return GGO_ERR_SHAPE;
@@ -757,7 +759,7 @@ int ggo_quantize_fp8_rows(const void* x_dev, int64_t rows, int64_t cols, int dty
 int ggo_quantize_mxfp8(const void* x_dev, int dtype, const int64_t* counts_dev, int num_segments,
                        int64_t rows, int64_t k, void* q_dev, void* scale_dev,
                        cudaStream_t stream) {
-  if (!x_dev || !counts_dev || !q_dev || !scale_dev || rows < 0 || k <= 0)
+  if (rows < 0 || k <= 0 || (rows > 0 && (!x_dev || !counts_dev || !q_dev || !scale_dev)))
     return GGO_ERR_INVALID_ARG;
   if (num_segments <= 0) return GGO_ERR_INVALID_ARG;
   if (num_segments > ggo::kMxMaxSegments) return GGO_ERR_TOO_MANY_SEGMENTS;
@@ -839,7 +841,8 @@ int ggo_moe_combine_checked(const void* y_sorted_dev, const float* topk_weights_
                             cudaStream_t stream) {
   // GgoWorkspace::error is the third int of the workspace
   const int* err = workspace_dev ? static_cast<const int*>(workspace_dev) + 2 : nullptr;
-  if (!y_sorted_dev || !topk_weights_dev || !slot_pos_dev || !out_dev) return GGO_ERR_INVALID_ARG;
+  if (num_tokens != 0 && (!y_sorted_dev || !topk_weights_dev || !slot_pos_dev || !out_dev))
+    return GGO_ERR_INVALID_ARG;
   if (num_tokens < 0 || hidden <= 0 || top_k <= 0 || top_k > ggo::kMaxTopK)
     return GGO_ERR_INVALID_ARG;
   if (dtype != GGO_DTYPE_BF16 && dtype != GGO_DTYPE_FP16) return GGO_ERR_DTYPE;
