@@ -179,8 +179,8 @@ int launch(const void* a, const void* b, int64_t b_rows, const GemmParams& p, in
 // up to 8) as find free SMs, while every one keeps four K steps and the mailbox holds their rows. The
 // tiles are estimated at one row block per expert that can have rows. A K step takes a CTA 0.2 us, the
 // cluster's start and the mail about 2.4 us and 0.06 a row: a split has to save more than it costs. In
-// one piece and split: 1 row, N = 512, K = 8192 18.2 and 10.5 us; 1 row, N = 4096, K = 14336 29.2 and
-// 20.7; 16 rows, N = K = 4096 13.3 and 12.8; 64 rows, N = 1024, K = 8192 22.3 and 18.4; against
+// one piece and split: 1 row, N = 512, K = 8192 17.9 and 10.5 us; 1 row, N = 4096, K = 14336 28.3 and
+// 19.8; 16 rows, N = K = 4096 12.2 and 11.2; 64 rows, N = 1024, K = 8192 21.8 and 18.5; against
 // it 60 rows, N = 4096, K = 2048 12.8 and 16.9.
 int split_parts(const GemmParams& p, int sms) {
   const int64_t blocks = p.rows < p.num_segments ? p.rows : p.num_segments;
@@ -498,8 +498,8 @@ int gemm_common(const void* input, const void* weights, void* output, const int6
   const bool bf16 = dtype == GGO_DTYPE_BF16;
   int bn = choose_bn(tile_config, rows, swiglu ? 2 * n : n, num_segments, g_sm_count[dev]);
   // int8: few rows over several experts are as many row blocks as experts, not rows / 128, and wide
-  // skinny tiles keep more weight bytes in flight. 16 rows over 8 experts, N = 14336, K = 4096: 78 us
-  // with 256-wide tiles, 83 us with 128; 16 rows of one expert, N = K = 4096: 17 and 13 us.
+  // skinny tiles keep more weight bytes in flight. 16 rows over 8 experts, N = 14336, K = 4096: 76 us
+  // with 256-wide tiles, 88 us with 128; 16 rows of one expert in one piece, N = K = 4096: 16 and 12.
   if (i8 && bn == 128 && tile_config == GGO_TILE_AUTO) {
     const int64_t blocks = rows < num_segments ? rows : num_segments;
     if (blocks * ((n + 255) / 256) >= g_sm_count[dev]) bn = 256;

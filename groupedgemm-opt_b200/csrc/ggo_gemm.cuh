@@ -128,8 +128,8 @@ struct TileInfo {
 
 // THIN: a launch of at most kSkinnyRows rows, whose tiles are all skinny: the A slot holds the skinny
 // box only, nothing is staged for TMA stores, and the room goes to more stages: 128 or 160 KB of
-// weights in flight instead of 96 or 128. 16 rows over 8 experts: N = 14336, K = 4096 85 -> 82 us,
-// N = 4096, K = 14336 81 -> 76 us, gate/up of F = 14336 149 -> 142 us.
+// weights in flight instead of 96 or 128. 16 rows over 8 experts: N = 14336, K = 4096 79 -> 76 us,
+// N = 4096, K = 14336 78 -> 75 us, gate/up of F = 14336 142 -> 139 us.
 // SPLIT (thin, 128 weight rows): a cluster of CTAs deals a tile's K steps out among them; the others'
 // integer sums arrive in the first one's mailbox, (cluster size - 1) x rows x 128 words.
 template <int BN, bool THIN = false, bool SPLIT = false>

@@ -139,7 +139,8 @@ __global__ void __launch_bounds__(256)
 }
 
 // One block of TB threads per row, the row held in registers, up to P 16-byte pieces a thread.
-// 32768 x 14336: 209 us, 6.7 TB/s, the rate of a plain copy. The sizes matter: 65536 x 4096 took 224 us
+// 32768 x 14336: 212 us at 1965 MHz (6.6 TB/s, the rate of a plain copy); 241 us (5.9 TB/s) in a stream
+// of calls that the power limit holds at 1640 MHz. The sizes matter: 65536 x 4096 took 224 us
 // with 256 threads and eight pieces, six of them idle, and takes 121 us.
 constexpr int kRegCols = 16384;
 

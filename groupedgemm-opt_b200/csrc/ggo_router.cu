@@ -245,9 +245,10 @@ __device__ __forceinline__ void route_block(const TL* __restrict__ logits,
 }
 
 // The first of two launches. grid = ceil(T / kTokens), NW warps: 8, or 32 (a token each) when the blocks
-// would not fill the GPU. table[b][e] and psum[b][e] receive block b's hist and its sum of P. Bound by
-// issue slots (70 % of them used, 580 instructions a token of 256 experts): 32768 x 256 in bf16 25 us,
-// of which reading takes 3.
+// would not fill the GPU. table[b][e] and psum[b][e] receive block b's hist and its sum of P. 32768 x 256
+// in bf16: 25 us, of which reading takes 3 and issuing the 580 instructions a token 16 (70 % of the issue
+// slots are used, 48 % of the warps resident); the rest is the wait of each of the k maxima for the one
+// before.
 template <typename TL, int V, bool VEC, int NW>
 __global__ void __launch_bounds__(32 * NW)
     router_kernel(const TL* __restrict__ logits, const uint8_t* __restrict__ mask, int T, int E,
@@ -333,8 +334,8 @@ __device__ __forceinline__ void write_totals(const ExpertScan& sc, int mine, int
 
 // The whole forward in one launch, for up to 8 x 32 tokens and 256 experts: one cluster, a block of 32
 // warps per 32 tokens, a token each. The blocks hand one another their counts and sums through
-// distributed shared memory and each writes its row of the offset table. 256 x 256 in fp32: 10.6 us, two
-// launches 12.6.
+// distributed shared memory and each writes its row of the offset table. 256 x 256 in fp32: 8.7 us; two
+// launches for one token more, 11.6.
 constexpr int kSmallBlocks = 8;
 template <typename TL, int V, bool VEC>
 __global__ void __launch_bounds__(1024)
@@ -485,7 +486,8 @@ __global__ void __launch_bounds__(1024)
 constexpr int kBwdWarps = 8;
 // Blocks that run at once on an SM (by registers). The grid is one wave of them: 32768 x 256 in bf16
 // 15.8 us, 18.1 us with a grid of 1.3 waves. The kernel issues 300 instructions a token, a third of
-// them in expf; its bytes would take 5 us.
+// them in expf, in 8 of its microseconds; its bytes would take 5. The rest is waiting: two warp sums
+// in a row for every token.
 constexpr int bwd_blocks(int v) { return v <= 8 ? 6 : (v == 16 ? 3 : 2); }
 
 template <typename TL, int V, bool VEC>

@@ -333,7 +333,7 @@ def fused_moe(
     timer: Optional[StageEvents] = None,
     routing: Optional[MoERouting] = None,
 ) -> torch.Tensor:
-    """MoE layer forward.
+    """MoE layer forward. Not differentiable (a given routing's weights are taken as values).
 
     Args:
         hidden: [T, H] bf16/fp16 tokens of this rank.

@@ -193,8 +193,10 @@ def grouped_gemm_opt_int8(
 ) -> torch.Tensor:
     """INT8 grouped GEMM: ``out[i] = (q_in[i] @ q_w[e(i)].T) * input_scale[i] * weight_scale[e(i)]``
     with signed 8-bit operands, exact 32-bit integer sums (tcgen05 kind::i8) and a bf16 or fp16
-    result (``out_dtype``), rounded once. Use :func:`quantize_int8` to produce the operands and
-    scales; one expert (``weights_q`` [1, N, K]) makes it a plain linear layer.
+    result (``out_dtype``). The sum is taken to fp32, multiplied by the two scales there (three
+    roundings, the first exact up to 2^24) and rounded once to the result's type. Use
+    :func:`quantize_int8` to produce the operands and scales; one expert (``weights_q`` [1, N, K])
+    makes it a plain linear layer.
 
     K a multiple of 16, at most 131056 (a longer sum could leave 32 bits); N a multiple of 8. Counts
     as in :func:`grouped_gemm_opt`; inside a CUDA-graph capture they must be on the GPU. Not

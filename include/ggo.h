@@ -169,8 +169,8 @@ int ggo_quantize_int8_rows(const void* x_dev, int64_t rows, int64_t cols, int dt
 /* INT8 grouped GEMM with one scale per row and per output channel:
  *   out[r, n] = (sum_k a[r,k] * b[e(r),n,k]) * input_scale[r] * weight_scale[e(r), n]
  * input_dev [T, K] and weights_dev [E, N, K] signed bytes, the sums exact 32-bit integers
- * (tcgen05 kind::i8), the two products with the scales in fp32, rounded once to out_dtype (bf16 or
- * fp16). swiglu != 0: weights_dev [E, 2N, K] holds N gate rows then N up rows, weight_scale_dev
+ * (tcgen05 kind::i8), taken to fp32 (exact up to 2^24), the two products with the scales in fp32 in
+ * that order, and one rounding to out_dtype (bf16 or fp16). swiglu != 0: weights_dev [E, 2N, K] holds N gate rows then N up rows, weight_scale_dev
  * [E, 2N], and out[r, n] = silu(gate) * up (N = F). Segment semantics as
  * ggo_grouped_gemm_segments. K a multiple of 16 and at most GGO_INT8_MAX_K (beyond it a sum of products
  * could leave 32 bits: GGO_ERR_SHAPE), N of 8. error_dev: a device word that receives device errors
