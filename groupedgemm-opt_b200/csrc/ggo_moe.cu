@@ -655,7 +655,8 @@ int dispatch_common(const void* x, int64_t num_tokens, int64_t hidden, int E, in
 extern "C" {
 
 size_t ggo_moe_route_scratch_bytes(int64_t num_tokens, int num_experts) {
-  if (num_tokens <= 0 || num_experts <= 0) return 16;
+  if (num_tokens < 0 || num_experts <= 0) return 16;
+  // one row of the table per block of tokens, then the experts' starts (without tokens too)
   return (static_cast<size_t>(ggo::nblocks_for(num_tokens)) + 1) * num_experts * sizeof(int);
 }
 

@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <array>
 #include <map>
+#include <memory>
 #include <mutex>
 #include <string>
 #include <tuple>
@@ -90,8 +91,8 @@ CapturedWorkspaces& captured_workspaces() {
 }
 
 struct CapturedLease {
-  int dev;
-  char* ws;
+  int dev = 0;
+  char* ws = nullptr;
 };
 
 void end_lease(void* p) {
@@ -106,7 +107,8 @@ void end_lease(void* p) {
 
 void* captured_workspace(const torch::Device& dev, cudaStream_t stream) {
   auto& all = captured_workspaces();
-  auto* lease = new CapturedLease{static_cast<int>(dev.index()), nullptr};
+  auto lease = std::make_unique<CapturedLease>();
+  lease->dev = static_cast<int>(dev.index());
   {
     std::lock_guard<std::mutex> lk(all.mu);
     auto& unused = all.unused[lease->dev];
@@ -128,9 +130,10 @@ void* captured_workspace(const torch::Device& dev, cudaStream_t stream) {
   const bool made =
       cudaStreamGetCaptureInfo(stream, &st, nullptr, &graph, nullptr, nullptr) == cudaSuccess &&
       st == cudaStreamCaptureStatusActive &&
-      cudaUserObjectCreate(&owner, lease, end_lease, 1, cudaUserObjectNoDestructorSync) ==
+      cudaUserObjectCreate(&owner, lease.get(), end_lease, 1, cudaUserObjectNoDestructorSync) ==
           cudaSuccess;
-  if (!made) end_lease(lease);
+  auto* given = lease.release();  // the object's, whose end gives the workspace back
+  if (!made) end_lease(given);
   TORCH_CHECK(made, "workspace of a captured call");
   if (cudaGraphRetainUserObject(graph, owner, 1, cudaGraphUserObjectMove) != cudaSuccess) {
     cudaUserObjectRelease(owner, 1);

@@ -33,6 +33,24 @@ def test_stages_without_tokens_need_no_addresses():
     assert f(None, 0, P, 8, 4, 128, P, P, None) == 1
 
 
+def test_route_scratch_without_tokens_holds_the_experts_starts():
+    f = ctypes.CDLL(str(lib_path())).ggo_moe_route_scratch_bytes
+    f.restype, f.argtypes = ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int]
+    assert f(0, 1024) == 4096 and f(0, 1) == 4 and f(1, 1024) == 8192
+
+
+@pytest.mark.gpu
+def test_routers_without_tokens():
+    """Counts of zero for every expert, and the experts' starts behind an empty table."""
+    from grouped_gemm_opt import _C, moe_router
+    for E in (1, 8, 1024):
+        l = torch.empty(0, E, device=DEV)
+        ids, w, tpe, scratch = _C.moe_route(l, 1)
+        assert ids.shape == w.shape == (0, 1) and tpe.tolist() == [0] * E
+        assert scratch.numel() == E and torch.all(scratch == 0)
+        assert moe_router(l, 1).tokens_per_expert.tolist() == [0] * E
+
+
 @pytest.mark.gpu
 def test_layers_without_tokens():
     import grouped_gemm_opt as ggo
