@@ -434,8 +434,7 @@ __device__ __forceinline__ float acc_to_float(uint32_t v) {
 // silu(gate) * up of two accumulator words under their scales. The integer path divides by
 // multiplying with the hardware reciprocal, within 2 ulp for divisors up to 2^126 (far below the
 // rounding to 16 bits that follows) and 0 beyond. Gates below -64, where 1 + e^-g is e^-g, take
-// g e^g u instead, as (g e^(g/2)) (u e^(g/2)): no factor leaves the normal numbers before the result
-// does.
+// g e^g u instead, as (g e^(g/2)) (u e^(g/2)), whose factors keep every bit that the result has.
 template <bool I8>
 __device__ __forceinline__ float scaled_silu_mul(uint32_t g, uint32_t u, float rs, float cg,
                                                  float cu) {

@@ -235,13 +235,13 @@ __global__ void __launch_bounds__(256)
     v[2 * i] = ok ? src[2 * c] : make_uint4(0, 0, 0, 0);
     v[2 * i + 1] = ok ? src[2 * c + 1] : make_uint4(0, 0, 0, 0);
   }
-  // the table's last row (the experts' starts) lies behind those of the blocks
-  const int* next = block_offsets + static_cast<size_t>(blockIdx.x + 1) * E;
+  const int* first = block_offsets + static_cast<size_t>(blockIdx.x) * E;
   const bool last = blockIdx.x + 1 == gridDim.x;
   for (int e = threadIdx.x; e < E; e += 256) {
-    off[e] = block_offsets[static_cast<size_t>(blockIdx.x) * E + e];
-    const int end = !last ? next[e] : (e + 1 < E ? next[e + 1] : T * K);
-    lim[e] = min(max(end, 0), T * K);
+    // the next block's first place or, behind the table's last block, the next expert's
+    const int begin = first[e], next = first[E + (last ? min(e + 1, E - 1) : e)];
+    off[e] = begin;
+    lim[e] = last && e + 1 == E ? T * K : min(max(next, 0), T * K);
   }
   __syncthreads();
   if (warp == 0) {

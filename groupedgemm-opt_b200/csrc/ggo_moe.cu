@@ -186,12 +186,12 @@ __global__ void __launch_bounds__(kRouteThreads)
   const int ntok = min(kRouteTokens, T - t0);
   const int nent = ntok * K;
   const bool last = blockIdx.x + 1 == gridDim.x;
+  const int* first = block_offsets + static_cast<size_t>(blockIdx.x) * E;
   for (int e = threadIdx.x; e < E; e += kRouteThreads) {
-    off[e] = block_offsets[static_cast<size_t>(blockIdx.x) * E + e];
-    const int end = !last       ? block_offsets[static_cast<size_t>(blockIdx.x + 1) * E + e]
-                    : e + 1 < E ? expert_start[e + 1]
-                                : T * K;
-    lim[e] = min(max(end, 0), T * K);
+    // the next block's first place or, behind the table's last block, the next expert's
+    const int at = first[e], next = first[E + (last ? min(e + 1, E - 1) : e)];
+    off[e] = at;
+    lim[e] = last && e + 1 == E ? T * K : min(max(next, 0), T * K);
     if (tg.world == 1) {
       delta[e] = 0;
     } else {
@@ -240,6 +240,16 @@ __global__ void __launch_bounds__(kRouteThreads)
     }
   }
   __syncthreads();
+  if (tg.world > 1) {
+    // Places of this block that no choice took (dropped ones leave them) hold a row of an earlier
+    // layer: its result goes to this place's own row on the source, which no choice reads. A block has
+    // at most 32 choices of an expert.
+    for (int e = threadIdx.x; e < E; e += kRouteThreads)
+      for (int ps = max(off[e], 0), n = 0; ps < lim[e] && n < kRouteTokens; ++ps, ++n) {
+        const long long to = static_cast<long long>(ps) + delta[e];
+        if (to >= 0 && to < tg.capacity) tg.origin[e / tg.el][to] = (tg.rank << 28) | ps;
+      }
+  }
   const int vec = H / 8;  // 16-byte chunks per row
   for (int tl = warp; tl < ntok; tl += kRouteThreads / 32) {
     const uint4* src = reinterpret_cast<const uint4*>(x + static_cast<size_t>(t0 + tl) * H);

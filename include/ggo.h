@@ -354,8 +354,8 @@ int ggo_ipc_free(void* ptr);
  * recv_rows[r] / recv_origin[r]: rank r's receive rows [capacity, H] and origin [capacity] int32,
  * as mapped in this process (own buffers for r == rank). Received rows are laid out
  * expert-major, [local expert][source rank], so each local expert is one contiguous segment;
- * recv_origin holds (source rank << 28) | the row's sorted position on its source rank.
- * slot_pos_dev and dropped choices as in ggo_moe_permute. */
+ * recv_origin holds (source rank << 28) | the row's sorted position on its source rank, also at a
+ * place that a dropped choice left empty. slot_pos_dev and dropped choices as in ggo_moe_permute. */
 int ggo_ep_dispatch(const void* x_dev, int64_t num_tokens, int64_t hidden, int num_experts,
                     int top_k, const int32_t* topk_ids_dev, const void* scratch_dev,
                     const int64_t* counts_all_dev, int world_size, int rank,

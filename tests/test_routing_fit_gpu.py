@@ -124,7 +124,8 @@ def test_edited_ids_make_their_tokens_nan_and_no_other():
 def test_peer_dispatch_stays_inside_the_buffers():
     """Counts that do not belong to the ids, as every rank publishes them: rows whose place lies behind
     the receive buffer are dropped, and the rows behind its end keep what they held. Where the counts
-    keep the experts' places apart, each place holds the row that its origin names."""
+    keep the experts' places apart, each place holds the row that its origin names. Places that dropped
+    choices left are named as their own."""
     from grouped_gemm_opt import _C
     T, H, E, k, cap = 100, 64, 8, 2, 230
     _, r = routing(T, E, k)
@@ -140,61 +141,122 @@ def test_peer_dispatch_stays_inside_the_buffers():
             org = [torch.full((cap + 400,), -5, dtype=torch.int32, device=DEV) for _ in range(2)]
             pos = _C.ep_dispatch(x, ids, r.scratch, counts.contiguous(), rank,
                                  [t.data_ptr() for t in recv], [t.data_ptr() for t in org], cap)
+            named = torch.cat([o[o != -5] & 0x0fffffff for o in org])
+            if ids is not r.topk_ids:  # all places lie in the buffer: every one is named once
+                assert torch.equal(named.sort()[0], torch.arange(T * k, device=DEV,
+                                                                 dtype=torch.int32))
             for a, o in zip(recv, org):
                 assert torch.all(a[cap:] == 7.0) and torch.all(o[cap:] == -5)
-                took = o[:cap] != -5
-                src = o[:cap][took] & 0x0fffffff
-                assert torch.all(o[:cap][took] >> 28 == rank) and int(src.numel()) <= T * k
+                word = o[:cap][o[:cap] != -5]
+                assert torch.all(word >> 28 == rank)
                 token = torch.full((T * k,), -1, dtype=torch.int64, device=DEV)
                 ok = pos >= 0
                 token[pos[ok].long()] = torch.arange(T, device=DEV).repeat_interleave(k)[ok]
-                assert not apart or torch.equal(a[:cap][took], x[token[src.long()]])
+                token = token[(word & 0x0fffffff).long()]
+                rows = a[:cap][o[:cap] != -5]
+                assert torch.all(rows[token < 0] == 7.0)
+                assert not apart or torch.equal(rows[token >= 0], x[token[token >= 0]])
 
 
-def test_peer_layer_with_a_given_routing():
-    """Two ranks of the peer-memory layer in turn: in the first pass rank 0 lacks rank 1's rows, in the
-    second every row and result has been delivered. The flags of both ranks are posted before each
-    call, so no kernel waits. The single-GPU layer adds up the same products, in tiles of other sizes:
-    an element of h, of y or of the result may round the other way, a step of 2^-7 each."""
-    from grouped_gemm_opt import _C, check_device_errors, fused_moe, moe_router
-    from grouped_gemm_opt.moe import _fused_moe_p2p
-    T, H, F, E, k, world = 40, 64, 128, 8, 2, 2
+class Ranks:
+    """The ranks of the peer-memory layer in one process, one after the other: `run` calls the layer of
+    every rank in turn with the flags of all posted before each call, so that no kernel waits. Rows
+    and results are complete after the second turn."""
+
+    def __init__(self, world, T, H, E, k):
+        from grouped_gemm_opt import _C
+        self.C, self.world, self.T, self.H, self.E, self.k = _C, world, T, H, E, k
+        self.cap = world * T * k
+        z = dict(device=DEV)
+        self.mem = {
+            "recv": [torch.zeros(self.cap, H, dtype=torch.bfloat16, **z) for _ in range(world)],
+            "origin": [torch.zeros(self.cap, dtype=torch.int32, **z) for _ in range(world)],
+            "back": [torch.zeros(T * k, H, dtype=torch.bfloat16, **z) for _ in range(world)],
+            "board": [torch.zeros(int(_C.ep_board_bytes(E)) // 8, dtype=torch.int64, **z)
+                      for _ in range(world)]}
+
+    def run(self, xs, ls, wgu, wd, rs):
+        from grouped_gemm_opt.moe import _fused_moe_p2p
+        ptrs = {n: [t.data_ptr() for t in ts] for n, ts in self.mem.items()}
+        el, outs = self.E // self.world, [None] * self.world
+        for _ in range(2):
+            for rank in range(self.world):
+                for b in self.mem["board"]:
+                    b[:self.world * self.E] = torch.stack([r.tokens_per_expert for r in rs]).flatten()
+                    b[8 * self.E:] = 1 << 40
+                bufs = SimpleNamespace(
+                    _C=self.C, world=self.world, rank=rank, max_tokens=self.T, hidden=self.H,
+                    top_k=self.k, num_experts=self.E, dtype=torch.bfloat16, epoch=0,
+                    capacity=self.cap, ptrs=ptrs, _own={n: p[rank] for n, p in ptrs.items()},
+                    wait_limit_cycles=1 << 24, recv=self.mem["recv"][rank],
+                    origin=self.mem["origin"][rank], back=self.mem["back"][rank],
+                    board_counts=self.mem["board"][rank][:8 * self.E].view(8, self.E))
+                local = slice(rank * el, (rank + 1) * el)
+                outs[rank] = _fused_moe_p2p(xs[rank], ls[rank], wgu[local], wd[local], self.k, bufs,
+                                            True, routing=rs[rank])
+        return outs
+
+
+def rank_inputs(world, T, H, F, E, k):
+    from grouped_gemm_opt import moe_router
     g = torch.Generator(device=DEV).manual_seed(0)
     wgu = (torch.randn(E, 2 * F, H, device=DEV, generator=g) * 0.1).to(torch.bfloat16)
     wd = (torch.randn(E, H, F, device=DEV, generator=g) * 0.1).to(torch.bfloat16)
     xs = [torch.randn(T, H, device=DEV, generator=g).to(torch.bfloat16) for _ in range(world)]
     ls = [torch.randn(T, E, device=DEV, generator=g) for _ in range(world)]
-    rs = [moe_router(l, k) for l in ls]
-    cap = world * T * k
-    mem = {"recv": [torch.zeros(cap, H, dtype=torch.bfloat16, device=DEV) for _ in range(world)],
-           "origin": [torch.zeros(cap, dtype=torch.int32, device=DEV) for _ in range(world)],
-           "back": [torch.zeros(T * k, H, dtype=torch.bfloat16, device=DEV) for _ in range(world)],
-           "board": [torch.zeros(int(_C.ep_board_bytes(E)) // 8, dtype=torch.int64, device=DEV)
-                     for _ in range(world)]}
-    ptrs = {n: [t.data_ptr() for t in ts] for n, ts in mem.items()}
-    el, outs = E // world, [None, None]
-    for _ in range(2):
-        for rank in range(world):
-            for b in mem["board"]:
-                b[:world * E] = torch.stack([r.tokens_per_expert for r in rs]).flatten()
-                b[8 * E:] = 1 << 40
-            bufs = SimpleNamespace(_C=_C, world=world, rank=rank, max_tokens=T, hidden=H, top_k=k,
-                                   num_experts=E, dtype=torch.bfloat16, epoch=0, capacity=cap,
-                                   ptrs=ptrs, _own={n: p[rank] for n, p in ptrs.items()},
-                                   wait_limit_cycles=1 << 24, recv=mem["recv"][rank],
-                                   origin=mem["origin"][rank], back=mem["back"][rank],
-                                   board_counts=mem["board"][rank][:8 * E].view(8, E))
-            local = slice(rank * el, (rank + 1) * el)
-            outs[rank] = _fused_moe_p2p(xs[rank], ls[rank], wgu[local], wd[local], k, bufs, True,
-                                        routing=rs[rank])
+    return xs, ls, wgu, wd, [moe_router(l, k) for l in ls]
+
+
+def other_rounding(x, wgu, wd, r, out):
+    """How far two layers over the same products may be apart that add them up in other orders: an
+    element of h, of y or of the result rounds the other way, a step of 2^-7 each."""
+    bound = 2.0 ** -7 * out.double().abs()
+    for j in range(r.topk_ids.size(1)):
+        e = r.topk_ids[:, j].long()
+        gate, up = torch.einsum("th,tfh->tf", x.double(), wgu[e].double()).chunk(2, 1)
+        h = (torch.nn.functional.silu(gate) * up).abs()
+        y = torch.einsum("tf,thf->th", h, wd[e].double().abs())  # at least |y|
+        bound += r.topk_weights[:, j, None].double() * 2 * 2.0 ** -7 * y
+    return bound
+
+
+@pytest.mark.parametrize("T", [40, 700])
+def test_peer_layer_with_a_given_routing(T):
+    """Equal to the single-GPU layer, whose tiles are of other sizes, but for roundings."""
+    from grouped_gemm_opt import check_device_errors, fused_moe
+    H, F, E, k, world = 64, 128, 8, 2, 2
+    xs, ls, wgu, wd, rs = rank_inputs(world, T, H, F, E, k)
+    outs = Ranks(world, T, H, E, k).run(xs, ls, wgu, wd, rs)
     check_device_errors(0)
     for rank in range(world):
-        want = fused_moe(xs[rank], ls[rank], wgu, wd, k, routing=rs[rank]).double()
-        bound = 2.0 ** -7 * want.abs()
-        for j in range(k):
-            e = rs[rank].topk_ids[:, j].long()
-            gate, up = torch.einsum("th,tfh->tf", xs[rank].double(), wgu[e].double()).chunk(2, 1)
-            h = (torch.nn.functional.silu(gate) * up).abs()
-            y = torch.einsum("tf,thf->th", h, wd[e].double().abs())  # at least |y|
-            bound += rs[rank].topk_weights[:, j, None].double() * 2 * 2.0 ** -7 * y
-        assert torch.all((outs[rank].double() - want).abs() <= bound)
+        want = fused_moe(xs[rank], ls[rank], wgu, wd, k, routing=rs[rank])
+        bound = other_rounding(xs[rank], wgu, wd, rs[rank], want)
+        assert torch.all((outs[rank].double() - want.double()).abs() <= bound)
+
+
+@pytest.mark.parametrize("T", [40, 700])
+def test_dropped_choices_in_the_peer_layer(T):
+    """The places that dropped choices leave in a peer's buffer hold a row of an earlier layer, whose
+    result must not be sent to where that row came from. The other tokens' rows may move up by a place,
+    no more."""
+    from grouped_gemm_opt import check_device_errors
+    H, F, E, k, world = 64, 128, 8, 2, 2
+    xs, ls, wgu, wd, rs = rank_inputs(world, T, H, F, E, k)
+    ranks = Ranks(world, T, H, E, k)
+    before = [o.clone() for o in ranks.run(xs, ls, wgu, wd, rs)]
+    cut, hit = [], []
+    for r in rs:
+        ids = r.topk_ids.clone()
+        drop = torch.zeros(T, dtype=torch.bool, device=DEV)
+        drop[[1, T // 2, T - 1]] = True
+        ids[1, 0], ids[T // 2, 1], ids[T - 1, 0] = -1, E, -9
+        cut.append(replace(r, topk_ids=ids))
+        hit.append(drop)
+    for b in ranks.mem["back"]:
+        b.fill_(float("nan"))  # results that nobody sends stay NaN
+    outs = ranks.run(xs, ls, wgu, wd, cut)
+    check_device_errors(0)
+    for x, r, out, want, drop in zip(xs, rs, outs, before, hit):
+        assert out[drop].isnan().all() and out[~drop].isfinite().all()
+        near = (out.double() - want.double()).abs() <= other_rounding(x, wgu, wd, r, want)
+        assert torch.all(near[~drop])
