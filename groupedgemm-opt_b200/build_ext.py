@@ -26,7 +26,7 @@ NVCC = str(CUDA_HOME / "bin" / "nvcc")
 
 CU_SOURCES = ["ggo_gemm.cu", "ggo_moe.cu", "ggo_router.cu", "ggo_int8.cu"]
 CU_HEADERS = ["ggo_gemm.cuh", "ggo_gemm_pair.cuh", "ggo_gemm_wgrad.cuh", "ggo_gemm_wgrad_pair.cuh",
-              "ggo_ptx.cuh", "ggo_order.cuh", "ggo_internal.h"]
+              "ggo_ptx.cuh", "ggo_internal.h"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 LIB_NAME = "libggo_b200.so"
 

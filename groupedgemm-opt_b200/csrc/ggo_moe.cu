@@ -1,21 +1,20 @@
-// Fused-MoE data-movement kernels: router top-k, deterministic permute/gather, weighted combine.
+// Fused-MoE data-movement kernels: deterministic permute/gather, weighted combine, row quantisers and
+// the expert-parallel exchange. The router is in ggo_router.cu.
 //
 // The reference has no router, permute or combine: its "fused MoE" entry point
 // (grouped_gemm_opt/triton_fused_moe.py:81-150) gathers through an identity `sorted_ids` and
 // computes the plain grouped GEMM. These kernels are the stages the layer needs around the
 // grouped GEMMs (ggo_gemm.cu), all stream-ordered and free of host synchronisation.
 //
-// Determinism: the only atomics are per-block expert histograms (order-independent sums). Sorted
-// positions come from per-block offsets (an exclusive scan over blocks) plus in-block ranks from
-// one warp walking the block's (token, slot) entries in order, so every position is a pure
-// function of the routing: expert-major, then token index.
+// Determinism: sorted positions come from the router's per-block offsets (an exclusive scan over
+// blocks) plus in-block ranks from one warp walking the block's (token, slot) entries in order, so
+// every position is a pure function of the routing: expert-major, then token index.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include "ggo.h"
 #include "ggo_internal.h"
-#include "ggo_order.cuh"
 
 namespace ggo {
 namespace {
@@ -25,127 +24,6 @@ constexpr int kMaxPeers = 8;       // expert-parallel ranks a dispatch can addre
 constexpr int kRouteThreads = 256;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopK = 16;
-
-// Top-k in the order of order_key (ties to the lower expert; key 0 marks an expert already chosen) and
-// the softmax over the chosen logits; weights 0 for a row of nothing but -inf.
-// grid = ceil(T / kRouteTokens); dynamic smem = (8 warps * E + E) * 4 bytes.
-__global__ void __launch_bounds__(kRouteThreads)
-    route_kernel(const float* __restrict__ logits, int T, int E, int K,
-                 int32_t* __restrict__ topk_ids, float* __restrict__ topk_w,
-                 int* __restrict__ block_counts) {
-  extern __shared__ uint32_t rsm[];
-  uint32_t* hist = rsm;                     // [E]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint32_t* keys = rsm + E + warp * E;      // [E] per warp
-  for (int e = threadIdx.x; e < E; e += kRouteThreads) hist[e] = 0;
-  __syncthreads();
-  const int t0 = blockIdx.x * kRouteTokens;
-  for (int tl = warp; tl < kRouteTokens; tl += kRouteThreads / 32) {
-    const int t = t0 + tl;
-    if (t >= T) break;
-    const float* row = logits + static_cast<size_t>(t) * E;
-    for (int e = lane; e < E; e += 32) keys[e] = order_key(row[e]);
-    __syncwarp();
-    float vals[kMaxTopK];
-    int ids[kMaxTopK];
-    for (int j = 0; j < K; ++j) {
-      // (key, lower index wins) packed so that a plain max picks the right element
-      unsigned long long best = 0;
-      for (int e = lane; e < E; e += 32) {
-        const unsigned long long c =
-            (static_cast<unsigned long long>(keys[e]) << 32) | (0xffffffffu - static_cast<uint32_t>(e));
-        best = c > best ? c : best;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-        best = other > best ? other : best;
-      }
-      const int id = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best & 0xffffffffu));
-      ids[j] = id;
-      vals[j] = order_value(static_cast<uint32_t>(best >> 32));
-      __syncwarp();
-      if (lane == 0) keys[id] = 0;
-      __syncwarp();
-    }
-    if (lane == 0) {
-      // softmax over the selected logits (vals[0] is the maximum)
-      const bool live = vals[0] != -INFINITY;
-      float s = 0.f, ex[kMaxTopK];
-      for (int j = 0; j < K; ++j) {
-        ex[j] = live ? expf(vals[j] - vals[0]) : 0.f;
-        s += ex[j];
-      }
-      const float inv = live ? 1.0f / s : 0.f;
-      for (int j = 0; j < K; ++j) {
-        topk_ids[static_cast<size_t>(t) * K + j] = ids[j];
-        topk_w[static_cast<size_t>(t) * K + j] = ex[j] * inv;
-        atomicAdd(&hist[ids[j]], 1u);
-      }
-    }
-    __syncwarp();
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < E; e += kRouteThreads)
-    block_counts[static_cast<size_t>(blockIdx.x) * E + e] = static_cast<int>(hist[e]);
-}
-
-// One block of 1024 threads. Turns block_counts[b][e] into absolute start rows (in place),
-// writes tokens_per_expert and the exclusive start row of every expert (expert_start[E], stored
-// right after the nblocks x E table). Each expert's column of the table is split into
-// P = 1024 / E contiguous block ranges, one per thread: range sums, a per-expert scan of the P
-// partial sums, a scan over experts, then every thread rewrites its range.
-__global__ void __launch_bounds__(1024)
-    route_scan_kernel(int* __restrict__ block_counts, int nblocks, int E,
-                      int64_t* __restrict__ tpe) {
-  __shared__ int part[1024];   // [E][P] range sums, then exclusive range offsets within expert
-  __shared__ int tot[kMaxExperts];
-  int* expert_start = block_counts + static_cast<size_t>(nblocks) * E;
-  const int P = max(1, 1024 / E);
-  const int tid = threadIdx.x;
-  const int e = tid / P, q = tid % P;
-  const bool active = e < E;
-  const int per = (nblocks + P - 1) / P;
-  const int b0 = min(nblocks, q * per), b1 = min(nblocks, b0 + per);
-  int sum = 0;
-  if (active)
-    for (int b = b0; b < b1; ++b) sum += block_counts[static_cast<size_t>(b) * E + e];
-  part[tid] = sum;
-  __syncthreads();
-  if (tid < E) {  // exclusive scan of expert tid's P range sums
-    int run = 0;
-    for (int j = 0; j < P; ++j) {
-      const int v = part[tid * P + j];
-      part[tid * P + j] = run;
-      run += v;
-    }
-    tot[tid] = run;
-  }
-  __syncthreads();
-  // exclusive scan over experts (E <= 1024): inclusive Hillis-Steele on a copy
-  __shared__ int inc[kMaxExperts];
-  if (tid < kMaxExperts) inc[tid] = tid < E ? tot[tid] : 0;
-  __syncthreads();
-  for (int o = 1; o < kMaxExperts; o <<= 1) {
-    const int v = (tid < kMaxExperts && tid >= o) ? inc[tid - o] : 0;
-    __syncthreads();
-    if (tid < kMaxExperts) inc[tid] += v;
-    __syncthreads();
-  }
-  if (tid < E) {
-    tpe[tid] = tot[tid];
-    expert_start[tid] = inc[tid] - tot[tid];
-  }
-  if (active) {
-    int run = inc[e] - tot[e] + part[tid];
-    for (int b = b0; b < b1; ++b) {
-      const size_t i = static_cast<size_t>(b) * E + e;
-      const int c = block_counts[i];
-      block_counts[i] = run;
-      run += c;
-    }
-  }
-}
 
 // Where dispatched rows go. world == 1: recv[0] is the local expert-sorted buffer and a row's
 // destination is its sorted position. world > 1 (expert parallelism): rank r owns experts
@@ -668,32 +546,6 @@ size_t ggo_moe_route_scratch_bytes(int64_t num_tokens, int num_experts) {
   if (num_tokens < 0 || num_experts <= 0) return 16;
   // one row of the table per block of tokens, then the experts' starts (without tokens too)
   return (static_cast<size_t>(ggo::nblocks_for(num_tokens)) + 1) * num_experts * sizeof(int);
-}
-
-int ggo_moe_route(const float* logits_dev, int64_t num_tokens, int num_experts, int top_k,
-                  int32_t* topk_ids_dev, float* topk_weights_dev,
-                  int64_t* tokens_per_expert_dev, void* scratch_dev, cudaStream_t stream) {
-  if (!tokens_per_expert_dev || !scratch_dev ||
-      (num_tokens != 0 && (!logits_dev || !topk_ids_dev || !topk_weights_dev)))
-    return GGO_ERR_INVALID_ARG;
-  if (num_tokens < 0 || num_experts <= 0 || num_experts > ggo::kMaxExperts || top_k <= 0 ||
-      top_k > ggo::kMaxTopK || top_k > num_experts)
-    return GGO_ERR_INVALID_ARG;
-  if (num_tokens * top_k > INT32_MAX) return GGO_ERR_SHAPE;
-  const int T = static_cast<int>(num_tokens);
-  const int nb = ggo::nblocks_for(T);
-  int* bc = static_cast<int*>(scratch_dev);
-  if (nb > 0) {
-    const size_t smem = static_cast<size_t>(num_experts) * (1 + ggo::kRouteThreads / 32) * 4;
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(ggo::route_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem)) != cudaSuccess)
-      return GGO_ERR_CUDA;
-    ggo::route_kernel<<<nb, ggo::kRouteThreads, smem, stream>>>(
-        logits_dev, T, num_experts, top_k, topk_ids_dev, topk_weights_dev, bc);
-  }
-  ggo::route_scan_kernel<<<1, 1024, 0, stream>>>(bc, nb, num_experts, tokens_per_expert_dev);
-  return ggo::check_launch();
 }
 
 int ggo_moe_permute(const void* x_dev, int64_t num_tokens, int64_t hidden, int num_experts,

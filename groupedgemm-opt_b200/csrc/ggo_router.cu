@@ -1,4 +1,4 @@
-// Router with balance loss, forward and backward.
+// Router, alone (ggo_moe_route) and with the balance loss, forward and backward.
 //
 // For every token t: the top_k experts of the fp32 logits l (ties to the lower index), their
 // softmax weights, and the softmax P over ALL experts. Over the kept tokens (not masked, at least
@@ -18,7 +18,6 @@
 
 #include "ggo.h"
 #include "ggo_internal.h"
-#include "ggo_order.cuh"
 
 namespace ggo {
 namespace {
@@ -27,6 +26,14 @@ constexpr int kTokens = 32;    // tokens per block: the granularity of the dispa
 constexpr int kMaxE = 1024;
 constexpr int kMaxK = 16;
 constexpr unsigned kAll = 0xffffffffu;
+
+// Monotone float -> uint32 (larger float -> larger key). -0 counts as +0 and NaN as the largest, so
+// that equal floats have equal keys; no float has key 0.
+__device__ __forceinline__ uint32_t order_key(float f) {
+  if (f != f) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(f + 0.0f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
 
 // A logit's key and its expert in one word, larger for larger logits and, among equal keys, for
 // lower experts, so that a plain maximum chooses. The 16-bit types' keys are whole (upper half);
@@ -181,7 +188,8 @@ __device__ __forceinline__ int choose_top_k(uint32_t (&k)[V], const TL* __restri
 // ids, weights and row_stat[t] = (max logit, 1 / sum exp(l - max)), the second 0 for tokens that are
 // not kept; in shared memory hist[e], the block's choices of expert e, all in the low and kept in the
 // high 16 bits, and wsum[warp][e], the warps' sums of P over kept tokens. Ends with a barrier.
-template <typename TL, int V, bool VEC, int NW>
+// Without LOSS: ids, weights and hist only.
+template <typename TL, int V, bool VEC, int NW, bool LOSS>
 __device__ __forceinline__ void route_block(const TL* __restrict__ logits,
                                             const uint8_t* __restrict__ mask, int T, int E, int K,
                                             int32_t* __restrict__ ids, float* __restrict__ weights,
@@ -222,7 +230,7 @@ __device__ __forceinline__ void route_block(const TL* __restrict__ logits,
     }
     // softmax over all experts
     float inv = 0.f;
-    if (kept) {
+    if (LOSS && kept) {
       float p[V];
       float z = 0.f;
 #pragma unroll
@@ -234,12 +242,14 @@ __device__ __forceinline__ void route_block(const TL* __restrict__ logits,
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[i] = fmaf(p[i], inv, acc[i]);
     }
-    if (lane == 0) row_stat[t] = make_float2(live ? top : 0.f, inv);
+    if (LOSS && lane == 0) row_stat[t] = make_float2(live ? top : 0.f, inv);
   }
+  if constexpr (LOSS) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int e = expert_of<V, VEC>(lane, i);
-    if (VEC || e < E) wsum[warp * E + e] = acc[i];
+    for (int i = 0; i < V; ++i) {
+      const int e = expert_of<V, VEC>(lane, i);
+      if (VEC || e < E) wsum[warp * E + e] = acc[i];
+    }
   }
   __syncthreads();
 }
@@ -249,7 +259,7 @@ __device__ __forceinline__ void route_block(const TL* __restrict__ logits,
 // in bf16: 25 us, of which reading takes 3 and issuing the 580 instructions a token 16 (70 % of the issue
 // slots are used, 48 % of the warps resident); the rest is the wait of each of the k maxima for the one
 // before.
-template <typename TL, int V, bool VEC, int NW>
+template <typename TL, int V, bool VEC, int NW, bool LOSS>
 __global__ void __launch_bounds__(32 * NW)
     router_kernel(const TL* __restrict__ logits, const uint8_t* __restrict__ mask, int T, int E,
                   int K, int32_t* __restrict__ ids, float* __restrict__ weights,
@@ -258,13 +268,15 @@ __global__ void __launch_bounds__(32 * NW)
   extern __shared__ uint32_t sm[];
   uint32_t* hist = sm;                                    // [E]
   float* wsum = reinterpret_cast<float*>(sm + E);         // [NW][E]
-  route_block<TL, V, VEC, NW>(logits, mask, T, E, K, ids, weights, row_stat, blockIdx.x * kTokens,
-                              hist, wsum);
+  route_block<TL, V, VEC, NW, LOSS>(logits, mask, T, E, K, ids, weights, row_stat,
+                                    blockIdx.x * kTokens, hist, wsum);
   for (int e = threadIdx.x; e < E; e += 32 * NW) {
-    float p = 0.f;
+    if constexpr (LOSS) {
+      float p = 0.f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) p += wsum[w * E + e];
-    psum[static_cast<size_t>(blockIdx.x) * E + e] = p;
+      for (int w = 0; w < NW; ++w) p += wsum[w * E + e];
+      psum[static_cast<size_t>(blockIdx.x) * E + e] = p;
+    }
     table[static_cast<size_t>(blockIdx.x) * E + e] = hist[e];
   }
 }
@@ -316,16 +328,19 @@ __device__ __forceinline__ ExpertScan scan_experts(int mine, int mine_kept, doub
 
 // loss = E sum_e (n_e / choices) (sum_t P / T'), T' = choices / K. The gradient takes f only through
 // f_e - sum P f, which a constant added to f does not change: coef_e = E (f_e - 1/E) / T', so that a
-// nearly balanced router's small gradient is not the difference of two large numbers.
+// nearly balanced router's small gradient is not the difference of two large numbers. Without LOSS: the
+// experts' counts only.
+template <bool LOSS>
 __device__ __forceinline__ void write_totals(const ExpertScan& sc, int mine, int mine_kept, int E,
                                              int K, int64_t* __restrict__ tpe,
                                              int64_t* __restrict__ kept_counts,
                                              float* __restrict__ loss, float* __restrict__ coef) {
   const int tid = threadIdx.x;
+  if (tid < E) tpe[tid] = mine;
+  if (!LOSS) return;
   const double n = static_cast<double>(sc.choices);
   const double scale = sc.choices > 0 ? static_cast<double>(E) * K / (n * n) : 0.0;
   if (tid < E) {
-    tpe[tid] = mine;
     kept_counts[tid] = mine_kept;
     coef[tid] = static_cast<float>(scale * (mine_kept - n / E));
   }
@@ -337,7 +352,7 @@ __device__ __forceinline__ void write_totals(const ExpertScan& sc, int mine, int
 // distributed shared memory and each writes its row of the offset table. 256 x 256 in fp32: 8.7 us; two
 // launches for one token more, 11.6.
 constexpr int kSmallBlocks = 8;
-template <typename TL, int V, bool VEC>
+template <typename TL, int V, bool VEC, bool LOSS>
 __global__ void __launch_bounds__(1024)
     router_small_kernel(const TL* __restrict__ logits, const uint8_t* __restrict__ mask, int T,
                         int E, int K, int32_t* __restrict__ ids, float* __restrict__ weights,
@@ -351,10 +366,10 @@ __global__ void __launch_bounds__(1024)
   unsigned rank, nblocks;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(nblocks));
-  route_block<TL, V, VEC, 32>(logits, mask, T, E, K, ids, weights, row_stat, rank * kTokens, hist,
-                              wsum);
+  route_block<TL, V, VEC, 32, LOSS>(logits, mask, T, E, K, ids, weights, row_stat, rank * kTokens,
+                                    hist, wsum);
   float p = 0.f;
-  if (tid < E) {
+  if (LOSS && tid < E) {
 #pragma unroll
     for (int w = 0; w < 32; ++w) p += wsum[w * E + tid];
   }
@@ -389,7 +404,7 @@ __global__ void __launch_bounds__(1024)
     table[rank * E + tid] = sc.start + before;
     if (rank == 0) table[nblocks * E + tid] = sc.start;
   }
-  if (rank == 0) write_totals(sc, all, kept, E, K, tpe, kept_counts, loss, coef);
+  if (rank == 0) write_totals<LOSS>(sc, all, kept, E, K, tpe, kept_counts, loss, coef);
 }
 
 // One cluster of up to 8 CTAs x 1024 threads; CTA r owns experts [r * CE, (r+1) * CE). Thread
@@ -397,7 +412,8 @@ __global__ void __launch_bounds__(1024)
 // a warp reads 32 neighbouring experts. R is at most 32: one thread per expert adds the ranges up. Totals are exchanged through distributed shared memory.
 // 32768 x 256: 15 us, the eight SMs' share of L2 bandwidth over two passes; 256 x 256: 5 us.
 // Turns table into the dispatch's absolute start rows (in place, expert starts right behind it) and
-// writes the counts, the loss and coef[e] = E (f_e - 1/E) / T' for the backward.
+// writes the counts and, with LOSS, the loss and coef[e] = E (f_e - 1/E) / T' for the backward.
+template <bool LOSS>
 __global__ void __launch_bounds__(1024)
     router_finish_kernel(uint32_t* __restrict__ table, const float* __restrict__ psum, int nblocks,
                          int E, int K, int CE, int CP, int64_t* __restrict__ tpe,
@@ -428,7 +444,7 @@ __global__ void __launch_bounds__(1024)
       const uint32_t v = table[static_cast<size_t>(b) * E + e];
       all += v & 0xffffu;
       kept += v >> 16;
-      p += psum[static_cast<size_t>(b) * E + e];
+      if (LOSS) p += psum[static_cast<size_t>(b) * E + e];
     }
   }
   part_all[tid] = all;
@@ -478,7 +494,7 @@ __global__ void __launch_bounds__(1024)
       run += v;
     }
   }
-  if (rank == 0) write_totals(sc, mine, mine_kept, E, K, tpe, kept_counts, loss, coef);
+  if (rank == 0) write_totals<LOSS>(sc, mine, mine_kept, E, K, tpe, kept_counts, loss, coef);
 }
 
 // One warp per token, persistent over tokens so that a lane's coefficients stay in registers. Every
@@ -577,11 +593,11 @@ bool vec_rows(const void* a, const void* b, int E) {
          ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15u) == 0;
 }
 
-template <typename TL, int V, bool VEC, int NW>
+template <typename TL, int V, bool VEC, int NW, bool LOSS>
 int launch_router_as(const void* logits, const uint8_t* mask, int T, int E, int K, int32_t* ids,
                      float* w, float2* stat, uint32_t* table, float* psum, cudaStream_t stream) {
   const size_t smem = static_cast<size_t>(E) * (1 + NW) * 4;  // at most 36 KB
-  router_kernel<TL, V, VEC, NW><<<blocks_for(T), 32 * NW, smem, stream>>>(
+  router_kernel<TL, V, VEC, NW, LOSS><<<blocks_for(T), 32 * NW, smem, stream>>>(
       static_cast<const TL*>(logits), mask, T, E, K, ids, w, stat, table, psum);
   return check_launch();
 }
@@ -590,27 +606,29 @@ int launch_router_as(const void* logits, const uint8_t* mask, int T, int E, int 
 // 256 tokens x 256 experts, fp32: 5.6 us against 16.5 us with eight warps of four tokens.
 constexpr int kWideBlocks = 148;
 
-template <typename TL, int V, bool VEC>
+template <typename TL, int V, bool VEC, bool LOSS>
 int launch_router_vec(const void* logits, const uint8_t* mask, int T, int E, int K, int32_t* ids,
                       float* w, float2* stat, uint32_t* table, float* psum, cudaStream_t stream) {
   if constexpr (V <= 8)
     if (blocks_for(T) <= kWideBlocks)
-      return launch_router_as<TL, V, VEC, 32>(logits, mask, T, E, K, ids, w, stat, table, psum,
-                                              stream);
-  return launch_router_as<TL, V, VEC, 8>(logits, mask, T, E, K, ids, w, stat, table, psum, stream);
+      return launch_router_as<TL, V, VEC, 32, LOSS>(logits, mask, T, E, K, ids, w, stat, table,
+                                                    psum, stream);
+  return launch_router_as<TL, V, VEC, 8, LOSS>(logits, mask, T, E, K, ids, w, stat, table, psum,
+                                               stream);
 }
 
-template <typename TL, int V>
+template <typename TL, int V, bool LOSS = true>
 int launch_router(const void* logits, const uint8_t* mask, int T, int E, int K, int32_t* ids,
                   float* w, float2* stat, uint32_t* table, float* psum, cudaStream_t stream) {
   if constexpr (V * sizeof(TL) >= 4)
     if (vec_rows<TL, V>(logits, nullptr, E))
-      return launch_router_vec<TL, V, true>(logits, mask, T, E, K, ids, w, stat, table, psum,
-                                            stream);
-  return launch_router_vec<TL, V, false>(logits, mask, T, E, K, ids, w, stat, table, psum, stream);
+      return launch_router_vec<TL, V, true, LOSS>(logits, mask, T, E, K, ids, w, stat, table, psum,
+                                                  stream);
+  return launch_router_vec<TL, V, false, LOSS>(logits, mask, T, E, K, ids, w, stat, table, psum,
+                                               stream);
 }
 
-template <typename TL, int V, bool VEC>
+template <typename TL, int V, bool VEC, bool LOSS>
 int launch_small_as(const void* logits, const uint8_t* mask, int T, int E, int K, int32_t* ids,
                     float* w, float2* stat, int* table, int64_t* tpe, int64_t* kept, float* loss,
                     float* coef, cudaStream_t stream) {
@@ -626,14 +644,14 @@ int launch_small_as(const void* logits, const uint8_t* mask, int T, int E, int K
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaError_t e = cudaLaunchKernelEx(&cfg, router_small_kernel<TL, V, VEC>,
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, router_small_kernel<TL, V, VEC, LOSS>,
                                          static_cast<const TL*>(logits), mask, T, E, K, ids, w,
                                          stat, table, tpe, kept, loss, coef))
     return cuda_fail(static_cast<int>(e));
   return check_launch();
 }
 
-template <typename TL, int V>
+template <typename TL, int V, bool LOSS = true>
 int launch_small(const void* logits, const uint8_t* mask, int T, int E, int K, int32_t* ids,
                  float* w, float2* stat, int* table, int64_t* tpe, int64_t* kept, float* loss,
                  float* coef, cudaStream_t stream) {
@@ -642,10 +660,10 @@ int launch_small(const void* logits, const uint8_t* mask, int T, int E, int K, i
   } else {
     if constexpr (V * sizeof(TL) >= 4)
       if (vec_rows<TL, V>(logits, nullptr, E))
-        return launch_small_as<TL, V, true>(logits, mask, T, E, K, ids, w, stat, table, tpe, kept,
-                                            loss, coef, stream);
-    return launch_small_as<TL, V, false>(logits, mask, T, E, K, ids, w, stat, table, tpe, kept,
-                                         loss, coef, stream);
+        return launch_small_as<TL, V, true, LOSS>(logits, mask, T, E, K, ids, w, stat, table, tpe,
+                                                  kept, loss, coef, stream);
+    return launch_small_as<TL, V, false, LOSS>(logits, mask, T, E, K, ids, w, stat, table, tpe,
+                                               kept, loss, coef, stream);
   }
 }
 
@@ -696,6 +714,50 @@ bool router_dtype_ok(int dtype) {
   return dtype == GGO_DTYPE_FP32 || dtype == GGO_DTYPE_BF16 || dtype == GGO_DTYPE_FP16;
 }
 
+// Routing without the loss, of fp32 logits.
+template <typename TL, int V>
+int launch_route(const void* logits, int T, int E, int K, int32_t* ids, float* w, uint32_t* table,
+                 cudaStream_t stream) {
+  return launch_router<TL, V, false>(logits, nullptr, T, E, K, ids, w, nullptr, table, nullptr,
+                                     stream);
+}
+
+template <typename TL, int V>
+int launch_route_small(const void* logits, int T, int E, int K, int32_t* ids, float* w,
+                       int* table, int64_t* tpe, cudaStream_t stream) {
+  return launch_small<TL, V, false>(logits, nullptr, T, E, K, ids, w, nullptr, table, tpe, nullptr,
+                                    nullptr, nullptr, stream);
+}
+
+// Whether one launch does the whole routing.
+bool small_routing(int nb, int E) { return nb > 0 && nb <= kSmallBlocks && E <= 256; }
+
+template <bool LOSS>
+int launch_finish(uint32_t* table, const float* psum, int nb, int E, int K, int64_t* tpe,
+                  int64_t* kept, float* loss, float* coef, cudaStream_t stream) {
+  // experts per CTA: 32 (a coalesced row piece), or E / 8 beyond 256 experts
+  int ncta = 1;
+  while (ncta < 8 && ncta * 32 < E) ncta *= 2;
+  const int CE = (E + ncta - 1) / ncta;
+  int CP = 1;
+  while (CP < CE) CP *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ncta, 1, 1);
+  cfg.blockDim = dim3(1024, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ncta;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, router_finish_kernel<LOSS>, table, psum, nb, E, K,
+                                         CE, CP, tpe, kept, loss, coef))
+    return cuda_fail(static_cast<int>(e));
+  return check_launch();
+}
+
 }  // namespace
 }  // namespace ggo
 
@@ -727,41 +789,44 @@ int ggo_moe_router(const void* logits_dev, int dtype, int64_t num_tokens, int nu
   const int nb = ggo::blocks_for(num_tokens);
   uint32_t* table = static_cast<uint32_t*>(scratch_dev);
   float* psum = reinterpret_cast<float*>(table + (static_cast<size_t>(nb) + 1) * E);
-  if (nb > 0 && nb <= ggo::kSmallBlocks && E <= 256)
+  float2* stat = reinterpret_cast<float2*>(row_stat_dev);
+  if (ggo::small_routing(nb, E))
     return GGO_ROUTER_CALL(ggo::launch_small, logits_dev, token_mask_dev, T, E, top_k,
-                           topk_ids_dev, topk_weights_dev,
-                           reinterpret_cast<float2*>(row_stat_dev),
-                           reinterpret_cast<int*>(table), tokens_per_expert_dev,
-                           balance_counts_dev, balance_loss_dev, coef_dev, stream);
+                           topk_ids_dev, topk_weights_dev, stat, reinterpret_cast<int*>(table),
+                           tokens_per_expert_dev, balance_counts_dev, balance_loss_dev, coef_dev,
+                           stream);
   if (nb > 0) {
     const int st = GGO_ROUTER_CALL(ggo::launch_router, logits_dev, token_mask_dev, T, E, top_k,
-                                   topk_ids_dev, topk_weights_dev,
-                                   reinterpret_cast<float2*>(row_stat_dev), table, psum, stream);
+                                   topk_ids_dev, topk_weights_dev, stat, table, psum, stream);
     if (st) return st;
   }
-  // experts per CTA: 32 (a coalesced row piece), or E / 8 beyond 256 experts
-  int ncta = 1;
-  while (ncta < 8 && ncta * 32 < E) ncta *= 2;
-  const int CE = (E + ncta - 1) / ncta;
-  int CP = 1;
-  while (CP < CE) CP *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ncta, 1, 1);
-  cfg.blockDim = dim3(1024, 1, 1);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ncta;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaError_t e = cudaLaunchKernelEx(&cfg, ggo::router_finish_kernel, table,
-                                         static_cast<const float*>(psum), nb, E, top_k, CE, CP,
-                                         tokens_per_expert_dev, balance_counts_dev,
-                                         balance_loss_dev, coef_dev))
-    return ggo::cuda_fail(static_cast<int>(e));
-  return ggo::check_launch();
+  return ggo::launch_finish<true>(table, psum, nb, E, top_k, tokens_per_expert_dev,
+                                  balance_counts_dev, balance_loss_dev, coef_dev, stream);
+}
+
+int ggo_moe_route(const float* logits_dev, int64_t num_tokens, int num_experts, int top_k,
+                  int32_t* topk_ids_dev, float* topk_weights_dev,
+                  int64_t* tokens_per_expert_dev, void* scratch_dev, cudaStream_t stream) {
+  if (!tokens_per_expert_dev || !scratch_dev ||
+      (num_tokens != 0 && (!logits_dev || !topk_ids_dev || !topk_weights_dev)))
+    return GGO_ERR_INVALID_ARG;
+  if (!ggo::router_args_ok(num_tokens, num_experts, top_k)) return GGO_ERR_INVALID_ARG;
+  if (num_tokens * top_k > INT32_MAX) return GGO_ERR_SHAPE;
+  if (reinterpret_cast<uintptr_t>(scratch_dev) & 3u) return GGO_ERR_ALIGNMENT;
+  const int T = static_cast<int>(num_tokens), E = num_experts;
+  const int nb = ggo::blocks_for(num_tokens);
+  uint32_t* table = static_cast<uint32_t*>(scratch_dev);
+  if (ggo::small_routing(nb, E))
+    return GGO_ROUTER_CALL_V(float, ggo::launch_route_small, logits_dev, T, E, top_k, topk_ids_dev,
+                             topk_weights_dev, reinterpret_cast<int*>(table),
+                             tokens_per_expert_dev, stream);
+  if (nb > 0) {
+    const int st = GGO_ROUTER_CALL_V(float, ggo::launch_route, logits_dev, T, E, top_k,
+                                     topk_ids_dev, topk_weights_dev, table, stream);
+    if (st) return st;
+  }
+  return ggo::launch_finish<false>(table, nullptr, nb, E, top_k, tokens_per_expert_dev, nullptr,
+                                   nullptr, nullptr, stream);
 }
 
 int ggo_moe_router_backward(const void* logits_dev, int dtype, int64_t num_tokens, int num_experts,
